@@ -19,6 +19,7 @@
 #include "elementwise.h"
 #include "gemm.h"
 #include "grpo.h"
+#include "head_loss_bindings.h"
 #include "moe.h"
 #include "kv_manager.h"
 #include "sampling.h"
@@ -1049,6 +1050,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("moe_dispatch", &moe_dispatch);
   m.def("moe_combine", &moe_combine);
   m.def("ep_exchange", &ep_exchange);
+  register_head_losses(m);
   m.def("set_pdl", [](bool on) { osb::pdl_enabled() = on; });
   m.def("attention_set_trace", [](c10::optional<Tensor> buf) {
     if (buf.has_value() && buf->defined()) {

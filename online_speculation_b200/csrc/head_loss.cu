@@ -1,0 +1,945 @@
+// Losses on a vocabulary head whose logits are never stored: softmax cross entropy and the
+// divergence from a teacher's listed logits, with the gradients of the hidden rows and of
+// the head.
+//
+//   l = h W^T,  q = softmax(it * l)                       h [R, H], W [V, H], bf16
+//   dl[r, v] = A_r q[r, v] - C_r on the unlisted columns, a stored value on the listed ones
+//   dh = dl W,  dW = dl^T h
+//
+// A row's listed columns are its target, or the teacher's columns; everything dense about
+// either loss is one row normaliser and two row coefficients.
+//
+// * Rows that do not count (ignored targets, empty lists) are taken out first: the products
+//   run over compact rows, so padding costs nothing and whatever its hidden rows hold never
+//   meets a product (0 * NaN would be NaN in dW).  The count stays on the device.
+// * Forward: the logits tile stays in tensor memory.  Lanes are rows, so a thread reduces its
+//   own row over the tile's columns (running maximum, sum of exponentials) without shuffles,
+//   and lifts the listed logits out on the way.  Listed columns are left out of the sum: the
+//   mass of the rest comes out of a sum of its own, not of 1 - (something near 1).
+// * Backward goes over pieces of the vocabulary.  A piece's logits are recomputed, turned into
+//   dl in bf16 (the type of the matrix instruction; 2^-9 rms against the same rounding of the
+//   outputs), and feed two products: dW of the piece is complete at once, dh adds up in fp32.
+//   Both read dl and their other operand in the layout they already have (MN-major
+//   shared-memory descriptors): nothing is transposed.
+#include "common.cuh"
+#include "head_loss.h"
+
+#include <algorithm>
+#include <climits>
+
+namespace osb {
+namespace {
+
+constexpr int kBM = 128;                  // accumulator rows (TMEM lanes)
+constexpr int kBN = 256;                  // accumulator columns
+constexpr int kBK = 64;                   // reduction elements a stage: one 128-byte swizzle row
+constexpr int kStages = 4;
+constexpr int kABytes = kBM * kBK * 2;
+constexpr int kBBytes = kBN * kBK * 2;
+constexpr int kStageBytes = kABytes + kBBytes;
+constexpr int kBox = 64 * 64 * 2;         // one MN-major box: 64 reduction rows of 64 elements
+constexpr int kOutBytes = 32 * 128;       // one warp's staged output box: 32 rows of 128 bytes
+constexpr int kThreads = 192;             // TMA warp, MMA warp, four epilogue warps
+constexpr int kSmem = 1024 + kStages * kStageBytes + 4 * 2 * kOutBytes + 256;
+constexpr float kLog2e = 1.4426950408889634f;
+
+enum Mode { kStats = 0, kGrad = 1, kProd = 2 };
+
+struct Maps {
+  CUtensorMap a0, b0;      // first kind: stats / grad operands, or the hidden gradient's
+  CUtensorMap a1, b1;      // second kind: the head gradient's
+  CUtensorMap out0, out1;
+};
+
+struct GemmArgs {
+  const int* count;
+  int H, V;
+  int v0, cols;            // this piece: first vocabulary row, columns that exist
+  int tiles_n;             // column tiles of the accumulator grid
+  int K;
+  const int* row_of;
+  const int* list_id;
+  float* list_logit;       // stats: written
+  const float* list_grad;  // grad: read
+  const float4* row_coef;  // grad
+  const float* inv_temp;   // stats
+  float2* part;
+  float* part_sum;
+  int part_tiles;
+  int rpad;
+  int do_dh, do_dw, splits, first_piece;
+  int* status;
+};
+
+// One work item: an accumulator tile and its range of reduction blocks.
+struct Item {
+  int kind;                // 0: first operand pair, 1: second
+  int m0, n0;
+  int kb0, kb1;
+  int split;
+};
+
+template <int MODE>
+__device__ __forceinline__ int item_count(const GemmArgs& a, int rows) {
+  const int tm = (rows + kBM - 1) / kBM;
+  if (MODE != kProd) return tm * a.tiles_n;
+  const int tv = (a.cols + kBM - 1) / kBM;
+  return (a.do_dh ? tm * a.tiles_n * a.splits : 0) + (a.do_dw ? tv * a.tiles_n : 0);
+}
+
+template <int MODE>
+__device__ __forceinline__ Item item_at(const GemmArgs& a, int rows, int w) {
+  Item it;
+  const int tm = (rows + kBM - 1) / kBM;
+  it.split = 0;
+  if (MODE != kProd) {
+    // rows fastest: the CTAs that run together read few head tiles, and the hidden rows stay in L2
+    it.kind = 0;
+    it.m0 = (w % tm) * kBM;
+    it.n0 = (w / tm) * kBN;
+    it.kb0 = 0;
+    it.kb1 = (a.H + kBK - 1) / kBK;
+    return it;
+  }
+  const int nh = a.do_dh ? tm * a.tiles_n * a.splits : 0;
+  if (w < nh) {
+    const int kb = (a.cols + kBK - 1) / kBK, per = (kb + a.splits - 1) / a.splits;
+    const int per_split = tm * a.tiles_n;
+    it.kind = 0;
+    it.split = w / per_split;
+    const int t = w % per_split;
+    it.m0 = (t / a.tiles_n) * kBM;
+    it.n0 = (t % a.tiles_n) * kBN;
+    it.kb0 = min(kb, it.split * per);
+    it.kb1 = min(kb, it.kb0 + per);
+  } else {
+    const int t = w - nh;
+    it.kind = 1;
+    it.m0 = (t / a.tiles_n) * kBM;
+    it.n0 = (t % a.tiles_n) * kBN;
+    it.kb0 = 0;
+    it.kb1 = (rows + kBK - 1) / kBK;
+  }
+  return it;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(smem_u32(src)), "r"(x), "r"(y)
+               : "memory");
+}
+
+__device__ __forceinline__ void tma_add_2d(const CUtensorMap* map, const void* src, int x, int y) {
+  asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(smem_u32(src)), "r"(x), "r"(y)
+               : "memory");
+}
+
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void bulk_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+
+// Position of 16-byte chunk c of row r in a 128-byte-swizzled box of 32 rows.
+__device__ __forceinline__ int swizzled(int r, int c) { return r * 128 + (((c ^ r) & 7) << 4); }
+
+// A row's cursor into its ascending list of columns.
+struct ListCursor {
+  const int* ids;
+  int k, K, next;
+  __device__ __forceinline__ void seek(const int* p, int count, int col) {
+    ids = p;
+    K = count;
+    int lo = 0, hi = count;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (ids[mid] < col) lo = mid + 1; else hi = mid;
+    }
+    k = lo;
+    next = k < K ? ids[k] : INT_MAX;
+  }
+  __device__ __forceinline__ void advance() {
+    ++k;
+    next = k < K ? ids[k] : INT_MAX;
+  }
+};
+
+template <int MODE>
+__global__ void __launch_bounds__(kThreads, 1)
+    head_gemm_kernel(const __grid_constant__ Maps maps, const GemmArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + kStages * kABytes;
+  uint8_t* sOut = smem + kStages * kStageBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sOut + 4 * 2 * kOutBytes);
+  uint64_t* empty = full + kStages;
+  uint64_t* tfull = empty + kStages;
+  uint64_t* tempty = tfull + 2;
+  uint64_t* drain = tempty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&tfull[i], 1);
+      mbar_init(&tempty[i], 4);
+    }
+    mbar_init(drain, 1);
+    fence_barrier_init();
+    fence_proxy_async_smem();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 2 * kBN);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_trigger();
+  pdl_wait();
+  const int rows = *a.count;
+  const int total = item_count<MODE>(a, rows);
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      int stage = 0, issued = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int w = blockIdx.x; w < total && ok; w += gridDim.x) {
+        const Item it = item_at<MODE>(a, rows, w);
+        for (int kb = it.kb0; kb < it.kb1; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1, a.status, kErrTmaWait)) {
+            ok = false;
+            break;
+          }
+          uint8_t* pa = sA + stage * kABytes;
+          uint8_t* pb = sB + stage * kBBytes;
+          mbar_arrive_expect_tx(&full[stage], kStageBytes);
+          if (MODE != kProd) {
+            tma_load_2d(pa, &maps.a0, kb * kBK, it.m0, &full[stage]);
+            tma_load_2d(pb, &maps.b0, kb * kBK, a.v0 + it.n0, &full[stage]);
+          } else if (it.kind == 0) {
+            tma_load_2d(pa, &maps.a0, kb * kBK, it.m0, &full[stage]);
+#pragma unroll
+            for (int j = 0; j < kBN / 64; ++j)
+              tma_load_2d(pb + j * kBox, &maps.b0, it.n0 + j * 64, a.v0 + kb * kBK, &full[stage]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < kBM / 64; ++j)
+              tma_load_2d(pa + j * kBox, &maps.a1, it.m0 + j * 64, kb * kBK, &full[stage]);
+#pragma unroll
+            for (int j = 0; j < kBN / 64; ++j)
+              tma_load_2d(pb + j * kBox, &maps.b1, it.n0 + j * 64, kb * kBK, &full[stage]);
+          }
+          ++issued;
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      if (!ok) {
+        // copies in flight land before the CTA may exit
+        for (int s = 0; s < kStages && s < issued; ++s) {
+          const int fills = (issued - s + kStages - 1) / kStages;
+          mbar_wait(&full[s], static_cast<uint32_t>((fills - 1) & 1), nullptr, 0);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      const uint32_t base_a = smem_u32(sA), base_b = smem_u32(sB);
+      for (int w = blockIdx.x; w < total && ok; w += gridDim.x) {
+        const Item it = item_at<MODE>(a, rows, w);
+        if (it.kb0 >= it.kb1) continue;
+        if (!mbar_wait(&tempty[acc], acc_phase ^ 1, a.status, kErrAccumWait)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d = tmem + acc * kBN;
+        const bool mn_a = MODE == kProd && it.kind == 1, mn_b = MODE == kProd;
+        const uint32_t idesc =
+            idesc_bf16_f32(kBM, kBN) | (mn_a ? 1u << 15 : 0u) | (mn_b ? 1u << 16 : 0u);
+        for (int kb = it.kb0; kb < it.kb1; ++kb) {
+          if (!mbar_wait(&full[stage], phase, a.status, kErrMmaWait)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t pa = base_a + stage * kABytes, pb = base_b + stage * kBBytes;
+#pragma unroll
+          for (int k = 0; k < kBK / 16; ++k) {
+            const uint64_t ad = mn_a ? sdesc_mn_sw128(pa + k * 2048, kBox, 1024) : sdesc_k_sw128(pa + k * 32);
+            const uint64_t bd = mn_b ? sdesc_mn_sw128(pb + k * 2048, kBox, 1024) : sdesc_k_sw128(pb + k * 32);
+            tc_mma_bf16(d, ad, bd, idesc, (kb > it.kb0 || k > 0) ? 1u : 0u);
+          }
+          tc_commit(&empty[stage]);
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        if (!ok) break;
+        tc_commit(&tfull[acc]);
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1;
+      }
+      // every issued MMA completes before TMEM is released
+      tc_commit(drain);
+      mbar_wait(drain, 0, a.status, kErrMmaWait);
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue
+    const int quarter = warp % 4;
+    const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+    uint8_t* out = sOut + quarter * 2 * kOutBytes;
+    int acc = 0, staged = 0;
+    uint32_t acc_phase = 0;
+    for (int w = blockIdx.x; w < total; w += gridDim.x) {
+      const Item it = item_at<MODE>(a, rows, w);
+      const int m = it.m0 + quarter * 32 + lane;
+      const bool empty_sum = it.kb0 >= it.kb1;
+      if (empty_sum && !(MODE == kProd && it.kind == 1)) continue;
+      // row inputs, fetched while the tile is still being multiplied
+      ListCursor cur;
+      long long list0 = 0;
+      float c2 = kLog2e;
+      float4 coef = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      bool live = false;
+      if (MODE != kProd) {
+        live = m < rows;
+        cur.k = 0;
+        cur.K = 0;
+        cur.next = INT_MAX;
+        if (live) {
+          const int o = a.row_of[m];
+          list0 = static_cast<long long>(o) * a.K;
+          if (MODE == kStats && a.inv_temp != nullptr) c2 = a.inv_temp[o] * kLog2e;
+          if (MODE == kGrad) coef = a.row_coef[m];
+          cur.seek(a.list_id + list0, a.K, a.v0 + it.n0);
+        }
+      }
+      if (!empty_sum) {
+        const bool ok = __all_sync(0xffffffffu, mbar_wait(&tfull[acc], acc_phase, a.status, kErrEpilogueWait));
+        if (!ok) break;
+        tc_fence_after();
+      }
+      const uint32_t t_acc = tmem + lane_base + acc * kBN;
+
+      if (MODE == kStats) {
+        float mx = -INFINITY, sum = 0.0f, plain = 0.0f;
+        for (int c = 0; c < kBN / 32; ++c) {
+          float x[32];
+          tmem_ld32(t_acc + c * 32, x);
+          const int col = a.v0 + it.n0 + c * 32;       // vocabulary column of x[0]
+          if (col >= a.V) break;
+          if (a.part_sum != nullptr) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) plain += x[j];   // columns behind V are zero
+          }
+          if (col + 32 > a.V) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (col + j >= a.V) x[j] = -INFINITY;
+          }
+          while (cur.next < col + 32) {
+            const int at = cur.next - col;
+            float v = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j == at) {
+                v = x[j];
+                x[j] = -INFINITY;
+              }
+            a.list_logit[list0 + cur.k] = v;
+            cur.advance();
+          }
+          __syncwarp();
+          float top = mx;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) top = fmaxf(top, x[j]);
+          const float ref = top == -INFINITY ? 0.0f : top;
+          sum *= ex2((mx - ref) * c2);
+          float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int j = 0; j < 32; ++j) s4[j & 3] += ex2((x[j] - ref) * c2);
+          sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+          mx = top;
+        }
+        if (live) {
+          const long long p = static_cast<long long>(m) * a.part_tiles + it.n0 / kBN;
+          a.part[p] = make_float2(mx, sum);
+          if (a.part_sum != nullptr) a.part_sum[p] = plain;
+        }
+      } else if (MODE == kGrad) {
+        // the whole tile is written: the products read its rows up to the tile's end
+        for (int c = 0; c < kBN / 64; ++c) {
+          uint8_t* box = out + (staged & 1) * kOutBytes;
+          if (lane == 0) bulk_wait_read<1>();
+          __syncwarp();
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            float x[32];
+            tmem_ld32(t_acc + c * 64 + half * 32, x);
+            const int col = a.v0 + it.n0 + c * 64 + half * 32;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) x[j] = coef.z * ex2(fmaf(x[j], coef.x, -coef.y)) - coef.w;
+            while (cur.next < col + 32) {
+              const int at = cur.next - col;
+              const float v = a.list_grad[list0 + cur.k];
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (j == at) x[j] = v;
+              cur.advance();
+            }
+            __syncwarp();
+            if (col + 32 > a.V) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (col + j >= a.V) x[j] = 0.0f;
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const uint4 v = make_uint4(pack2(x[8 * q], x[8 * q + 1]), pack2(x[8 * q + 2], x[8 * q + 3]),
+                                         pack2(x[8 * q + 4], x[8 * q + 5]), pack2(x[8 * q + 6], x[8 * q + 7]));
+              *reinterpret_cast<uint4*>(box + swizzled(lane, half * 4 + q)) = v;
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&maps.out0, box, it.n0 + c * 64, it.m0 + quarter * 32);
+            bulk_commit();
+          }
+          ++staged;
+        }
+      } else if (it.kind == 0) {
+        // hidden gradient: fp32, added to what earlier pieces left
+        for (int c = 0; c < kBN / 32; ++c) {
+          float x[32];
+          tmem_ld32(t_acc + c * 32, x);
+          if (it.n0 + c * 32 >= a.H) break;
+          uint8_t* box = out + (staged & 1) * kOutBytes;
+          if (lane == 0) bulk_wait_read<1>();
+          __syncwarp();
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            *reinterpret_cast<float4*>(box + swizzled(lane, q)) =
+                make_float4(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            const int y = it.split * a.rpad + it.m0 + quarter * 32;
+            if (a.first_piece)
+              tma_store_2d(&maps.out0, box, it.n0 + c * 32, y);
+            else
+              tma_add_2d(&maps.out0, box, it.n0 + c * 32, y);
+            bulk_commit();
+          }
+          ++staged;
+        }
+      } else {
+        // head gradient of the piece: complete, rounded once
+        const bool in_rows = a.v0 + it.m0 + quarter * 32 < a.V;
+        for (int c = 0; c < kBN / 64; ++c) {
+          if (it.n0 + c * 64 >= a.H) break;
+          uint8_t* box = out + (staged & 1) * kOutBytes;
+          if (lane == 0) bulk_wait_read<1>();
+          __syncwarp();
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            float x[32];
+            if (empty_sum) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) x[j] = 0.0f;
+            } else {
+              tmem_ld32(t_acc + c * 64 + half * 32, x);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const uint4 v = make_uint4(pack2(x[8 * q], x[8 * q + 1]), pack2(x[8 * q + 2], x[8 * q + 3]),
+                                         pack2(x[8 * q + 4], x[8 * q + 5]), pack2(x[8 * q + 6], x[8 * q + 7]));
+              *reinterpret_cast<uint4*>(box + swizzled(lane, half * 4 + q)) = v;
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            // a group for every box, stored or not: the waits above count groups
+            if (in_rows) tma_store_2d(&maps.out1, box, it.n0 + c * 64, a.v0 + it.m0 + quarter * 32);
+            bulk_commit();
+          }
+          ++staged;
+        }
+      }
+      if (!empty_sum) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tempty[acc]);
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1;
+      }
+    }
+    if (lane == 0) bulk_wait_all();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 2 * kBN);
+  }
+}
+
+// ------------------------------------------------------------------ rows ----
+__device__ __forceinline__ long long load_id(const void* p, int i64, long long i) {
+  return i64 ? static_cast<const long long*>(p)[i] : static_cast<const int*>(p)[i];
+}
+
+// The teacher's list of one row (one warp): empty slots dropped, a column listed twice
+// merged, ascending by column; its masses in fp64, rounded to fp32.
+__global__ void __launch_bounds__(128) teacher_rows_kernel(const HeadLossState s, const HeadTargets t) {
+  extern __shared__ uint8_t raw[];
+  pdl_trigger();
+  pdl_wait();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int K = s.K;
+  double* mass = reinterpret_cast<double*>(raw) + static_cast<long long>(warp) * K;
+  int* id = reinterpret_cast<int*>(raw + static_cast<long long>(4) * K * 8) + warp * K;
+  int* key = id + 4 * K;
+  const int r = blockIdx.x * 4 + warp;
+  if (r >= s.R) return;
+  const long long base = static_cast<long long>(r) * K;
+  const double it = s.inv_temp != nullptr ? static_cast<double>(s.inv_temp[r]) : 1.0;
+  double top = -INFINITY;
+  bool any = false, nan = false;
+  for (int k = lane; k < K; k += 32) {
+    long long v = load_id(t.ids, t.ids_i64, base + k);
+    const float x = t.teacher_bf16 ? bf2f(static_cast<const __nv_bfloat16*>(t.teacher)[base + k])
+                                   : static_cast<const float*>(t.teacher)[base + k];
+    if (v >= s.V) {
+      record_error(s.status, kErrBadIndex);
+      v = -1;
+    }
+    const bool has = v >= 0 && !(x == -INFINITY);
+    id[k] = has ? static_cast<int>(v) : INT_MAX;
+    const double z = has ? static_cast<double>(x) * it : -INFINITY;
+    mass[k] = z;
+    any |= has;
+    nan |= has && !(z == z);
+    top = fmax(top, z);
+  }
+  any = __any_sync(0xffffffffu, any);
+  nan = __any_sync(0xffffffffu, nan);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const double shift = t.teacher_lse != nullptr ? static_cast<double>(t.teacher_lse[r]) : top;
+  __syncwarp();
+  double sum = 0.0;
+  for (int k = lane; k < K; k += 32) {
+    const double e = id[k] == INT_MAX ? 0.0 : exp(mass[k] - shift);
+    mass[k] = e;
+    sum += e;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const double inv = t.teacher_lse != nullptr ? 1.0 : 1.0 / sum;
+  __syncwarp();
+  // first slot of every column takes the masses of its later ones
+  for (int k = lane; k < K; k += 32) {
+    const int v = id[k];
+    bool first = v != INT_MAX;
+    for (int j = 0; j < k && first; ++j) first = id[j] != v;
+    key[k] = first ? v : INT_MAX;
+  }
+  __syncwarp();
+  for (int k = lane; k < K; k += 32) s.list_id[base + k] = INT_MAX;
+  __syncwarp();
+  for (int k = lane; k < K; k += 32) {
+    const int v = key[k];
+    if (v == INT_MAX) continue;
+    int at = 0;
+    double m = mass[k];
+    for (int j = 0; j < K; ++j) {
+      at += key[j] < v;
+      if (j > k && id[j] == v) m += mass[j];
+    }
+    s.list_id[base + at] = v;
+    s.list_mass[base + at] = static_cast<float>(m * inv);
+  }
+  if (lane == 0) {
+    t.active[r] = any ? 1 : 0;
+    const double rest = t.teacher_lse != nullptr ? (nan ? sum : fmax(1.0 - sum, 0.0)) : 0.0;
+    s.rest_mass[r] = static_cast<float>(rest);
+  }
+}
+
+// Numbers the rows that count (one block); a target outside the vocabulary is recorded and
+// its row left out.
+__global__ void __launch_bounds__(1024) compact_rows_kernel(const HeadLossState s, const HeadTargets t) {
+  __shared__ int warp_sums[32];
+  __shared__ int carry;
+  pdl_trigger();
+  pdl_wait();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (threadIdx.x == 0) carry = 0;
+  __syncthreads();
+  for (int r0 = 0; r0 < s.R; r0 += 1024) {
+    const int r = r0 + threadIdx.x;
+    bool on = false;
+    if (r < s.R) {
+      if (s.divergence) {
+        on = t.active[r] != 0;
+      } else {
+        const long long v = load_id(t.ids, t.ids_i64, r);
+        on = v != t.ignore_index;
+        if (on && (v < 0 || v >= s.V)) {
+          record_error(s.status, kErrBadIndex);
+          on = false;
+        }
+        s.list_id[r] = on ? static_cast<int>(v) : INT_MAX;
+      }
+    }
+    const unsigned ballot = __ballot_sync(0xffffffffu, on);
+    if (lane == 0) warp_sums[warp] = __popc(ballot);
+    __syncthreads();
+    int before = carry;
+    for (int q = 0; q < warp; ++q) before += warp_sums[q];
+    const int m = before + __popc(ballot & ((1u << lane) - 1u));
+    if (r < s.R) {
+      s.compact_of[r] = on ? m : -1;
+      if (on) s.row_of[m] = r;
+      else s.loss[r] = 0.0f;
+    }
+    __syncthreads();
+    if (threadIdx.x == 1023) carry = before + __popc(ballot);
+    __syncthreads();
+  }
+  const int n = carry;
+  for (int m = n + threadIdx.x; m < s.rpad; m += 1024) s.row_of[m] = -1;
+  if (threadIdx.x == 0) *s.count = n;
+}
+
+__global__ void __launch_bounds__(128) gather_rows_kernel(const HeadLossState s) {
+  pdl_trigger();
+  pdl_wait();
+  const int m = blockIdx.x;
+  const int n = *s.count;
+  if (m >= (n + kHeadRowPad - 1) / kHeadRowPad * kHeadRowPad) return;
+  const int vecs = s.H / 8;
+  uint4* dst = reinterpret_cast<uint4*>(s.hc + static_cast<long long>(m) * s.H);
+  if (m >= n) {
+    for (int i = threadIdx.x; i < vecs; i += 128) dst[i] = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  const uint4* src = reinterpret_cast<const uint4*>(s.h + static_cast<long long>(s.row_of[m]) * s.ldh);
+  for (int i = threadIdx.x; i < vecs; i += 128) dst[i] = src[i];
+}
+
+__device__ __forceinline__ double warp_sum_f64(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Folds the tiles of a row and forms its loss (one warp a row).  The normaliser and the loss
+// are formed in fp64 from fp32 sums: a divergence is a small difference of logarithms.
+__global__ void __launch_bounds__(128) finish_rows_kernel(const HeadLossState s, const HeadStatsScratch p) {
+  pdl_trigger();
+  pdl_wait();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int m = blockIdx.x * 4 + warp;
+  if (m >= *s.count) return;
+  const int r = s.row_of[m];
+  const float itf = s.inv_temp != nullptr ? s.inv_temp[r] : 1.0f;
+  const double it = itf;
+  const float c2 = itf * kLog2e;
+  const float2* part = p.part + static_cast<long long>(m) * p.tiles;
+  float mx = -INFINITY;
+  for (int i = lane; i < p.tiles; i += 32) mx = fmaxf(mx, part[i].x);
+  mx = warp_max(mx);
+  double rest = 0.0, plain = 0.0;
+  for (int i = lane; i < p.tiles; i += 32) {
+    const float2 v = part[i];
+    if (v.x != -INFINITY || !(v.y == 0.0f)) rest += static_cast<double>(v.y) * exp2f((v.x - mx) * c2);
+    if (p.part_sum != nullptr) plain += p.part_sum[static_cast<long long>(m) * p.tiles + i];
+  }
+  rest = warp_sum_f64(rest);
+  if (p.part_sum != nullptr) plain = warp_sum_f64(plain);
+  const long long base = static_cast<long long>(r) * s.K;
+  float top = mx;
+  for (int k = lane; k < s.K; k += 32)
+    if (s.list_id[base + k] != INT_MAX) top = fmaxf(top, s.list_logit[base + k]);
+  top = warp_max(top);
+  double listed = 0.0;
+  for (int k = lane; k < s.K; k += 32)
+    if (s.list_id[base + k] != INT_MAX)
+      listed += exp((static_cast<double>(s.list_logit[base + k]) - static_cast<double>(top)) * it);
+  listed = warp_sum_f64(listed);
+  if (mx != -INFINITY) rest *= exp((static_cast<double>(mx) - static_cast<double>(top)) * it);
+  const double total = rest + listed;
+  const double lse = static_cast<double>(top) * it + log(total);
+  const double q_rest = rest / total;
+  double loss, factor;
+  if (!s.divergence) {
+    const double target = s.list_logit[base];
+    const double hot = listed > 0.0 ? log1p(rest / listed) : lse - target;
+    const double eps = s.smoothing;
+    loss = (1.0 - eps) * hot + s.z_loss * lse * lse;
+    if (p.part_sum != nullptr) loss += eps * (lse - plain / s.V);
+    factor = 1.0 + 2.0 * s.z_loss * lse;
+  } else {
+    double sum = 0.0;
+    for (int k = lane; k < s.K; k += 32) {
+      if (s.list_id[base + k] == INT_MAX) continue;
+      const double mass = s.list_mass[base + k];
+      if (mass == 0.0) continue;
+      sum += mass * (log(mass) - (static_cast<double>(s.list_logit[base + k]) * it - lse));
+    }
+    loss = warp_sum_f64(sum);
+    factor = 1.0;
+    const double rest_mass = s.rest_bucket ? static_cast<double>(s.rest_mass[r]) : 0.0;
+    // a list of all columns leaves no rest; a teacher mass there is rounding
+    if (s.rest_bucket && rest_mass != 0.0 && rest > 0.0) {
+      loss += rest_mass * log(rest_mass / q_rest);
+      factor = 1.0 - rest_mass / q_rest;
+    }
+  }
+  if (lane == 0) {
+    s.loss[r] = static_cast<float>(loss);
+    s.row_stat[r] = make_float4(static_cast<float>(lse), static_cast<float>(q_rest), static_cast<float>(factor), 0.0f);
+  }
+}
+
+// Row coefficients and listed values of the logits' gradient (one warp a compact row).
+__global__ void __launch_bounds__(128) grad_rows_kernel(const HeadLossState s, const HeadGradArgs g) {
+  pdl_trigger();
+  pdl_wait();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int m = blockIdx.x * 4 + warp;
+  if (m >= s.rpad) return;
+  if (m >= *s.count) {
+    // rows behind the last of its tile: zero whatever the tile holds there
+    if (lane == 0) g.row_coef[m] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    return;
+  }
+  const int r = s.row_of[m];
+  const float4 st = s.row_stat[r];
+  const float it = s.inv_temp != nullptr ? s.inv_temp[r] : 1.0f;
+  const float up = g.g[r] * it;
+  const float flat = s.divergence ? 0.0f : s.smoothing / static_cast<float>(s.V);
+  if (lane == 0) g.row_coef[m] = make_float4(it * kLog2e, st.x * kLog2e, up * st.z, up * flat);
+  const long long base = static_cast<long long>(r) * s.K;
+  for (int k = lane; k < s.K; k += 32) {
+    if (s.list_id[base + k] == INT_MAX) continue;
+    float v;
+    if (s.divergence) {
+      v = expf(s.list_logit[base + k] * it - st.x) - s.list_mass[base + k];
+    } else {
+      // a p - 1 with p - 1 = -(mass of the rest): no cancellation in sure rows
+      v = (st.z - 1.0f) * (1.0f - st.y) - st.y + s.smoothing - flat;
+    }
+    g.list_grad[base + k] = up * v;
+  }
+}
+
+__global__ void __launch_bounds__(128) hidden_grad_kernel(const HeadLossState s, const HeadGradArgs g) {
+  pdl_trigger();
+  pdl_wait();
+  const int r = blockIdx.x;
+  const int m = s.compact_of[r];
+  const int vecs = s.H / 8;
+  uint4* dst = reinterpret_cast<uint4*>(g.dh + static_cast<long long>(r) * s.H);
+  for (int i = threadIdx.x; i < vecs; i += 128) {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (m >= 0) {
+      float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+      for (int q = 0; q < g.splits; ++q) {
+        const float4* src = reinterpret_cast<const float4*>(
+            g.dh_part + (static_cast<long long>(q) * s.rpad + m) * s.H + i * 8);
+        const float4 lo = __ldcg(src), hi = __ldcg(src + 1);
+        x[0] += lo.x; x[1] += lo.y; x[2] += lo.z; x[3] += lo.w;
+        x[4] += hi.x; x[5] += hi.y; x[6] += hi.z; x[7] += hi.w;
+      }
+      v = make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7]));
+    }
+    dst[i] = v;
+  }
+}
+
+// ------------------------------------------------------------------ host ----
+bool encode(CUtensorMap* map, CUtensorMapDataType type, int size, const void* ptr, long long rows, long long cols,
+            long long ld, int box_cols, int box_rows) {
+  EncodeTiledFn fn = tensor_map_encoder();
+  if (!fn) return false;
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * size};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
+  cuuint32_t estr[2] = {1, 1};
+  return fn(map, type, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool map_bf16(CUtensorMap* map, const void* ptr, long long rows, long long cols, long long ld, int box_cols,
+              int box_rows) {
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, ptr, rows, cols, ld, box_cols, box_rows);
+}
+
+int device_sms() {
+  static int cached[64] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (!cached[dev]) {
+    int n = 0;
+    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    cached[dev] = n > 0 ? n : 148;
+  }
+  return cached[dev];
+}
+
+template <int MODE>
+cudaError_t launch_gemm(const Maps& maps, const GemmArgs& a, int max_items, cudaStream_t stream) {
+  static bool set[64] = {false};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 64 || !set[dev]) {
+    e = cudaFuncSetAttribute(head_gemm_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) set[dev] = true;
+  }
+  const int grid = std::max(1, std::min(max_items, device_sms()));
+  return launch_pdl(head_gemm_kernel<MODE>, dim3(grid), dim3(kThreads), kSmem, stream, maps, a);
+}
+
+GemmArgs base_args(const HeadLossState& s) {
+  GemmArgs a{};
+  a.count = s.count;
+  a.H = s.H;
+  a.V = s.V;
+  a.K = s.K;
+  a.row_of = s.row_of;
+  a.list_id = s.list_id;
+  a.rpad = s.rpad;
+  a.status = s.status;
+  return a;
+}
+
+int ceil_div(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
+
+}  // namespace
+
+int head_loss_vocab_tiles(int V) { return ceil_div(V, kBN); }
+
+int head_loss_piece(int rpad, int V) {
+  long long piece = (128ll << 20) / (2ll * rpad) / kBN * kBN;
+  piece = std::max<long long>(piece, 4096);
+  return static_cast<int>(std::min<long long>(piece, static_cast<long long>(ceil_div(V, kBN)) * kBN));
+}
+
+int head_loss_splits(int R, int H, int piece, int V) {
+  const int tiles = ceil_div(R, kBM) * ceil_div(H, kBN);
+  const int kb = ceil_div(std::min(piece, V), kBK);
+  const int want = std::max(1, std::min({device_sms() / std::max(1, tiles), kb / 4, 32}));
+  const int per = ceil_div(kb, want);
+  return ceil_div(kb, per);
+}
+
+cudaError_t head_loss_rows_launch(const HeadLossState& s, const HeadTargets& t, cudaStream_t stream) {
+  cudaError_t e;
+  if (s.divergence) {
+    const size_t smem = static_cast<size_t>(4) * s.K * (8 + 4 + 4);
+    e = launch_pdl(teacher_rows_kernel, dim3(ceil_div(s.R, 4)), dim3(128), smem, stream, s, t);
+    if (e != cudaSuccess) return e;
+  }
+  e = launch_pdl(compact_rows_kernel, dim3(1), dim3(1024), 0, stream, s, t);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(gather_rows_kernel, dim3(s.rpad), dim3(128), 0, stream, s);
+}
+
+cudaError_t head_loss_forward_launch(const HeadLossState& s, const HeadStatsScratch& p, cudaStream_t stream) {
+  Maps maps{};
+  if (!map_bf16(&maps.a0, s.hc, s.rpad, s.H, s.H, kBK, kBM)) return cudaErrorInvalidValue;
+  if (!map_bf16(&maps.b0, s.w, s.V, s.H, s.ldw, kBK, kBN)) return cudaErrorInvalidValue;
+  GemmArgs a = base_args(s);
+  a.v0 = 0;
+  a.cols = s.V;
+  a.tiles_n = ceil_div(s.V, kBN);
+  a.list_logit = s.list_logit;
+  a.inv_temp = s.inv_temp;
+  a.part = p.part;
+  a.part_sum = p.part_sum;
+  a.part_tiles = p.tiles;
+  cudaError_t e = launch_gemm<kStats>(maps, a, ceil_div(s.R, kBM) * a.tiles_n, stream);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(finish_rows_kernel, dim3(ceil_div(s.R, 4)), dim3(128), 0, stream, s, p);
+}
+
+cudaError_t head_loss_backward_launch(const HeadLossState& s, const HeadGradArgs& g, cudaStream_t stream) {
+  cudaError_t e = launch_pdl(grad_rows_kernel, dim3(ceil_div(s.rpad, 4)), dim3(128), 0, stream, s, g);
+  if (e != cudaSuccess) return e;
+  Maps gm{}, pm{};
+  const bool dh = g.dh != nullptr, dw = g.dw != nullptr;
+  if (!map_bf16(&gm.a0, s.hc, s.rpad, s.H, s.H, kBK, kBM) || !map_bf16(&gm.b0, s.w, s.V, s.H, s.ldw, kBK, kBN) ||
+      !map_bf16(&gm.out0, g.dl, s.rpad, g.piece, g.piece, 64, 32))
+    return cudaErrorInvalidValue;
+  if (dh && (!map_bf16(&pm.a0, g.dl, s.rpad, g.piece, g.piece, kBK, kBM) ||
+             !map_bf16(&pm.b0, s.w, s.V, s.H, s.ldw, 64, kBK) ||
+             !encode(&pm.out0, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, g.dh_part,
+                     static_cast<long long>(g.splits) * s.rpad, s.H, s.H, 32, 32)))
+    return cudaErrorInvalidValue;
+  if (dw && (!map_bf16(&pm.a1, g.dl, s.rpad, g.piece, g.piece, 64, kBK) ||
+             !map_bf16(&pm.b1, s.hc, s.rpad, s.H, s.H, 64, kBK) ||
+             !map_bf16(&pm.out1, g.dw, s.V, s.H, s.H, 64, 32)))
+    return cudaErrorInvalidValue;
+  for (int v0 = 0; v0 < s.V; v0 += g.piece) {
+    GemmArgs a = base_args(s);
+    a.v0 = v0;
+    a.cols = std::min(g.piece, s.V - v0);
+    a.tiles_n = ceil_div(a.cols, kBN);
+    a.list_grad = g.list_grad;
+    a.row_coef = g.row_coef;
+    e = launch_gemm<kGrad>(gm, a, ceil_div(s.R, kBM) * a.tiles_n, stream);
+    if (e != cudaSuccess) return e;
+    a.tiles_n = ceil_div(s.H, kBN);
+    a.do_dh = dh;
+    a.do_dw = dw;
+    a.splits = g.splits;
+    a.first_piece = v0 == 0;
+    const int items = (dh ? ceil_div(s.R, kBM) * a.tiles_n * g.splits : 0) +
+                      (dw ? ceil_div(a.cols, kBM) * a.tiles_n : 0);
+    e = launch_gemm<kProd>(pm, a, items, stream);
+    if (e != cudaSuccess) return e;
+  }
+  if (dh) return launch_pdl(hidden_grad_kernel, dim3(s.R), dim3(128), 0, stream, s, g);
+  return cudaSuccess;
+}
+
+}  // namespace osb

@@ -1,0 +1,250 @@
+// PyTorch bindings of the vocabulary-head losses and the top logits (head_loss.cu, top_logits.cu).
+//
+// Scratch and saved tensors come from PyTorch's allocator on every call: two graphs, or two
+// streams, never share them.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include "head_loss.h"
+#include "head_loss_bindings.h"
+#include "top_logits.h"
+
+namespace {
+
+using torch::Tensor;
+using OptTensor = c10::optional<Tensor>;
+
+void check(cudaError_t e, const char* what) {
+  TORCH_CHECK(e == cudaSuccess, what, " failed: ", cudaGetErrorString(e));
+}
+
+bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
+
+// Rows the tile loads can address: unit inner stride, 16-byte aligned starts.  Others are copied.
+Tensor tile_rows(const Tensor& t) {
+  const bool ok = t.stride(1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 &&
+                  (t.size(0) == 1 || (t.stride(0) >= t.size(1) && t.stride(0) % 8 == 0));
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+long long row_stride(const Tensor& t) { return t.size(0) == 1 ? t.size(1) : t.stride(0); }
+
+void check_matrix(const Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.dim() == 2 && t.scalar_type() == torch::kBFloat16, name, " must be a 2-D CUDA bf16 tensor");
+}
+
+// Per-row state of one call, carved out of one byte buffer (saved for the backward pass).
+struct Carve {
+  char* base;
+  size_t at = 0;
+  template <typename T>
+  T* take(long long n) {
+    T* p = reinterpret_cast<T*>(base + at);
+    at += (static_cast<size_t>(n) * sizeof(T) + 255) / 256 * 256;
+    return p;
+  }
+};
+
+size_t bind_state(osb::HeadLossState& s, char* base) {
+  Carve c{base};
+  const long long listed = static_cast<long long>(s.R) * s.K;
+  s.hc = c.take<__nv_bfloat16>(static_cast<long long>(s.rpad) * s.H);
+  s.row_of = c.take<int>(s.rpad);
+  s.compact_of = c.take<int>(s.R);
+  s.count = c.take<int>(1);
+  s.list_id = c.take<int>(listed);
+  s.list_logit = c.take<float>(listed);
+  s.list_mass = c.take<float>(s.divergence ? listed : 0);
+  s.rest_mass = c.take<float>(s.divergence ? s.R : 0);
+  s.row_stat = c.take<float4>(s.R);
+  return c.at;
+}
+
+osb::HeadLossState make_state(const Tensor& w, int64_t R, int64_t H, int64_t K, const OptTensor& inv_temp,
+                              bool divergence, bool rest_bucket, double smoothing, double z_loss, const Tensor& status) {
+  TORCH_CHECK(R >= 1 && H >= 8 && H % 8 == 0, "hidden rows must be a multiple of 8 wide");
+  TORCH_CHECK(w.size(0) >= 1 && w.size(0) < (1ll << 31) - 65536 && R < (1ll << 31) - 65536, "too many rows");
+  TORCH_CHECK(K >= 1 && K <= osb::kHeadMaxListed, "listed columns per row: 1 to ", osb::kHeadMaxListed);
+  TORCH_CHECK(status.is_cuda() && status.scalar_type() == torch::kInt32, "status word");
+  osb::HeadLossState s{};
+  s.R = static_cast<int>(R);
+  s.H = static_cast<int>(H);
+  s.V = static_cast<int>(w.size(0));
+  s.K = static_cast<int>(K);
+  s.rpad = static_cast<int>((R + osb::kHeadRowPad - 1) / osb::kHeadRowPad * osb::kHeadRowPad);
+  s.w = reinterpret_cast<const __nv_bfloat16*>(w.data_ptr());
+  s.ldw = row_stride(w);
+  s.divergence = divergence;
+  s.rest_bucket = rest_bucket;
+  s.smoothing = static_cast<float>(smoothing);
+  s.z_loss = static_cast<float>(z_loss);
+  s.status = status.data_ptr<int>();
+  if (given(inv_temp)) {
+    TORCH_CHECK(inv_temp->is_cuda() && inv_temp->scalar_type() == torch::kFloat32 && inv_temp->is_contiguous() &&
+                    inv_temp->numel() == R,
+                "inv_temp needs one contiguous float per row");
+    s.inv_temp = inv_temp->data_ptr<float>();
+  }
+  return s;
+}
+
+// ids [R] (cross entropy) or [R, K] with teacher logits [R, K].  Returns (loss [R], saved bytes).
+std::tuple<Tensor, Tensor> head_loss_forward(Tensor h, Tensor weight, Tensor ids, OptTensor teacher,
+                                             OptTensor teacher_lse, OptTensor inv_temp, int64_t ignore_index,
+                                             double smoothing, double z_loss, Tensor status) {
+  check_matrix(h, "h");
+  check_matrix(weight, "weight");
+  TORCH_CHECK(h.size(1) == weight.size(1) && h.device() == weight.device(), "h and weight differ in width or device");
+  TORCH_CHECK(ids.is_cuda() && ids.device() == h.device() && ids.is_contiguous(), "ids must be contiguous on the device of h");
+  TORCH_CHECK(ids.scalar_type() == torch::kInt32 || ids.scalar_type() == torch::kInt64, "ids must be int32 or int64");
+  const int64_t R = h.size(0), H = h.size(1);
+  const bool divergence = given(teacher);
+  TORCH_CHECK(ids.dim() == (divergence ? 2 : 1) && ids.size(0) == R, "one row of ids for every row of h");
+  const int64_t K = divergence ? ids.size(1) : 1;
+  c10::cuda::CUDAGuard guard(h.device());
+  const Tensor rows = tile_rows(h), w = tile_rows(weight);
+  osb::HeadLossState s = make_state(w, R, H, K, inv_temp, divergence, given(teacher_lse), smoothing, z_loss, status);
+  const auto bytes = h.options().dtype(torch::kUInt8), floats = h.options().dtype(torch::kFloat32);
+  Tensor saved = torch::empty({static_cast<int64_t>(bind_state(s, nullptr))}, bytes);
+  bind_state(s, static_cast<char*>(saved.data_ptr()));
+  s.h = reinterpret_cast<const __nv_bfloat16*>(rows.data_ptr());
+  s.ldh = row_stride(rows);
+  Tensor loss = torch::empty({R}, floats);
+  s.loss = loss.data_ptr<float>();
+
+  osb::HeadTargets t{};
+  t.ids = ids.data_ptr();
+  t.ids_i64 = ids.scalar_type() == torch::kInt64;
+  t.ignore_index = ignore_index;
+  if (divergence) {
+    TORCH_CHECK(teacher->is_cuda() && teacher->is_contiguous() && teacher->sizes() == ids.sizes(),
+                "teacher logits must be contiguous and shaped like ids");
+    TORCH_CHECK(teacher->scalar_type() == torch::kFloat32 || teacher->scalar_type() == torch::kBFloat16,
+                "teacher logits must be fp32 or bf16");
+    t.teacher = teacher->data_ptr();
+    t.teacher_bf16 = teacher->scalar_type() == torch::kBFloat16;
+    if (given(teacher_lse)) {
+      TORCH_CHECK(teacher_lse->is_cuda() && teacher_lse->scalar_type() == torch::kFloat32 &&
+                      teacher_lse->is_contiguous() && teacher_lse->numel() == R,
+                  "teacher_lse needs one contiguous float per row");
+      t.teacher_lse = teacher_lse->data_ptr<float>();
+    }
+  }
+  osb::HeadStatsScratch p{};
+  p.tiles = osb::head_loss_vocab_tiles(s.V);
+  const long long parts = static_cast<long long>(s.rpad) * p.tiles;
+  Carve size{nullptr};
+  size.take<float2>(parts);
+  size.take<float>(smoothing != 0.0 ? parts : 0);
+  size.take<unsigned char>(R);
+  Tensor scratch = torch::empty({static_cast<int64_t>(size.at)}, bytes);
+  Carve c{static_cast<char*>(scratch.data_ptr())};
+  p.part = c.take<float2>(parts);
+  float* part_sum = c.take<float>(smoothing != 0.0 ? parts : 0);
+  p.part_sum = smoothing != 0.0 ? part_sum : nullptr;
+  t.active = c.take<unsigned char>(R);
+  const auto stream = at::cuda::getCurrentCUDAStream();
+  check(osb::head_loss_rows_launch(s, t, stream), "head loss rows");
+  check(osb::head_loss_forward_launch(s, p, stream), "head loss forward");
+  return {loss, saved};
+}
+
+// Gradients of sum_r g[r] loss[r]: (dh [R, H] or undefined, dW [V, H] or undefined), bf16.
+std::tuple<OptTensor, OptTensor> head_loss_backward(Tensor saved, Tensor weight, OptTensor inv_temp, Tensor g,
+                                                    int64_t K, bool divergence, bool rest_bucket, double smoothing,
+                                                    double z_loss, bool need_dh, bool need_dw, int64_t piece,
+                                                    Tensor status) {
+  check_matrix(weight, "weight");
+  TORCH_CHECK(g.is_cuda() && g.scalar_type() == torch::kFloat32 && g.is_contiguous() && g.dim() == 1, "g: one float per row");
+  const int64_t R = g.size(0), H = weight.size(1), V = weight.size(0);
+  c10::cuda::CUDAGuard guard(weight.device());
+  const Tensor w = tile_rows(weight);
+  osb::HeadLossState s = make_state(w, R, H, K, inv_temp, divergence, rest_bucket, smoothing, z_loss, status);
+  TORCH_CHECK(saved.scalar_type() == torch::kUInt8 && saved.numel() == static_cast<int64_t>(bind_state(s, nullptr)),
+              "saved state does not belong to these arguments");
+  bind_state(s, static_cast<char*>(saved.data_ptr()));
+  osb::HeadGradArgs a{};
+  a.g = g.data_ptr<float>();
+  if (piece > 0) {
+    TORCH_CHECK(piece % 256 == 0, "pieces are multiples of 256 columns");
+    a.piece = static_cast<int>(std::min<int64_t>(piece, (V + 255) / 256 * 256));
+  } else {
+    a.piece = osb::head_loss_piece(s.rpad, s.V);
+  }
+  a.splits = need_dh ? osb::head_loss_splits(s.R, s.H, a.piece, s.V) : 1;
+  const auto opts = weight.options();
+  OptTensor dh, dw;
+  if (need_dh) {
+    dh = torch::empty({R, H}, opts);
+    a.dh = reinterpret_cast<__nv_bfloat16*>(dh->data_ptr());
+  }
+  if (need_dw) {
+    dw = torch::empty({V, H}, opts);
+    a.dw = reinterpret_cast<__nv_bfloat16*>(dw->data_ptr());
+  }
+  const long long dl = static_cast<long long>(s.rpad) * a.piece;
+  const long long parts = need_dh ? static_cast<long long>(a.splits) * s.rpad * H : 0;
+  Carve size{nullptr};
+  size.take<__nv_bfloat16>(dl);
+  size.take<float>(parts);
+  size.take<float4>(s.rpad);
+  size.take<float>(R * K);
+  Tensor scratch = torch::empty({static_cast<int64_t>(size.at)}, opts.dtype(torch::kUInt8));
+  Carve c{static_cast<char*>(scratch.data_ptr())};
+  a.dl = c.take<__nv_bfloat16>(dl);
+  a.dh_part = c.take<float>(parts);
+  a.row_coef = c.take<float4>(s.rpad);
+  a.list_grad = c.take<float>(R * K);
+  check(osb::head_loss_backward_launch(s, a, at::cuda::getCurrentCUDAStream()), "head loss backward");
+  return {dh, dw};
+}
+
+std::tuple<Tensor, Tensor, Tensor> top_logits(Tensor logits, int64_t k, OptTensor inv_temp) {
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.stride(1) == 1, "logits must be 2-D CUDA rows of unit inner stride");
+  TORCH_CHECK(logits.scalar_type() == torch::kFloat32 || logits.scalar_type() == torch::kBFloat16, "logits must be fp32 or bf16");
+  const int64_t R = logits.size(0), V = logits.size(1);
+  TORCH_CHECK(R >= 1 && k >= 1 && k <= V && k <= osb::kTopLogitsMax && V < (1ll << 31) - 65536, "top_logits sizes");
+  osb::TopLogitsArgs a{};
+  if (given(inv_temp)) {
+    TORCH_CHECK(inv_temp->is_cuda() && inv_temp->scalar_type() == torch::kFloat32 && inv_temp->is_contiguous() &&
+                    inv_temp->numel() == R,
+                "inv_temp needs one contiguous float per row");
+    a.inv_temp = inv_temp->data_ptr<float>();
+  }
+  c10::cuda::CUDAGuard guard(logits.device());
+  const auto floats = logits.options().dtype(torch::kFloat32);
+  Tensor values = torch::empty({R, k}, floats), ids = torch::empty({R, k}, floats.dtype(torch::kInt32));
+  Tensor lse = torch::empty({R}, floats);
+  a.logits = logits.data_ptr();
+  a.bf16 = logits.scalar_type() == torch::kBFloat16;
+  a.ld = row_stride(logits);
+  a.V = static_cast<int>(V);
+  a.k = static_cast<int>(k);
+  a.splits = osb::top_logits_splits(static_cast<int>(std::min<int64_t>(R, 1 << 20)), a.V, a.k);
+  TORCH_CHECK(R * a.splits < (1ll << 31), "too many rows");
+  a.R = static_cast<int>(R);
+  a.values = values.data_ptr<float>();
+  a.ids = ids.data_ptr<int>();
+  a.lse = lse.data_ptr<float>();
+  Tensor scratch;
+  if (a.splits > 1) {
+    Carve size{nullptr};
+    size.take<unsigned long long>(R * a.splits * k);
+    size.take<float2>(R * a.splits);
+    scratch = torch::empty({static_cast<int64_t>(size.at)}, floats.dtype(torch::kUInt8));
+    Carve c{static_cast<char*>(scratch.data_ptr())};
+    a.keys = c.take<unsigned long long>(R * a.splits * k);
+    a.part = c.take<float2>(R * a.splits);
+  }
+  check(osb::top_logits_launch(a, at::cuda::getCurrentCUDAStream()), "top logits");
+  return {values, ids, lse};
+}
+
+}  // namespace
+
+void register_head_losses(pybind11::module_& m) {
+  m.def("head_loss_forward", &head_loss_forward);
+  m.def("head_loss_backward", &head_loss_backward);
+  m.def("top_logits", &top_logits);
+}

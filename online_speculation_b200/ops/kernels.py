@@ -14,6 +14,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _ext, workspace
+from .head_loss import head_cross_entropy, head_topk_divergence, top_logits  # noqa: F401  (public entry points)
 
 PAGE_SIZE = 32
 HEAD_DIM = 128
