@@ -30,12 +30,13 @@
 namespace osb {
 namespace {
 
-constexpr int kBM = 128;                  // accumulator rows (TMEM lanes)
-constexpr int kBN = 256;                  // accumulator columns
+constexpr int kBM = 256;                  // tile rows: 128 TMEM lanes in each CTA of the pair
+constexpr int kBN = 256;                  // tile columns: both CTAs hold all of them for their rows
+constexpr int kHalf = 128;                // rows of A, and of B, that one CTA stages
 constexpr int kBK = 64;                   // reduction elements a stage: one 128-byte swizzle row
-constexpr int kStages = 4;
-constexpr int kABytes = kBM * kBK * 2;
-constexpr int kBBytes = kBN * kBK * 2;
+constexpr int kStages = 6;
+constexpr int kABytes = kHalf * kBK * 2;
+constexpr int kBBytes = kHalf * kBK * 2;
 constexpr int kStageBytes = kABytes + kBBytes;
 constexpr int kBox = 64 * 64 * 2;         // one MN-major box: 64 reduction rows of 64 elements
 constexpr int kOutBytes = 32 * 128;       // one warp's staged output box: 32 rows of 128 bytes
@@ -123,6 +124,39 @@ __device__ __forceinline__ Item item_at(const GemmArgs& a, int rows, int w) {
   return it;
 }
 
+// ------------------------------------------------------------- CTA pairs ----
+// Loads into this CTA's shared memory that complete on a barrier of the pair's first CTA.
+__device__ __forceinline__ void pair_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], "
+      "[%4];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+
+__device__ __forceinline__ void pair_mma(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                         uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Arrives on the barrier at this offset in both CTAs when the MMAs issued so far are done.
+__device__ __forceinline__ void pair_commit(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+
+__device__ __forceinline__ void remote_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -180,7 +214,7 @@ struct ListCursor {
 };
 
 template <int MODE>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     head_gemm_kernel(const __grid_constant__ Maps maps, const GemmArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -194,6 +228,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* drain = tempty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int rank = static_cast<int>(cluster_ctarank());
+  const int pair = blockIdx.x / 2, pairs = gridDim.x / 2;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -202,18 +238,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tfull[i], 1);
-      mbar_init(&tempty[i], 4);
+      mbar_init(&tempty[i], 8);   // the epilogue warps of both CTAs
     }
     mbar_init(drain, 1);
     fence_barrier_init();
     fence_proxy_async_smem();
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, 2 * kBN);
-    tmem_relinquish();
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(2 * kBN)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
+  cluster_sync();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_trigger();
@@ -227,7 +266,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int stage = 0, issued = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int w = blockIdx.x; w < total && ok; w += gridDim.x) {
+      for (int w = pair; w < total && ok; w += pairs) {
         const Item it = item_at<MODE>(a, rows, w);
         for (int kb = it.kb0; kb < it.kb1; ++kb) {
           if (!mbar_wait(&empty[stage], phase ^ 1, a.status, kErrTmaWait)) {
@@ -236,22 +275,24 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           uint8_t* pa = sA + stage * kABytes;
           uint8_t* pb = sB + stage * kBBytes;
-          mbar_arrive_expect_tx(&full[stage], kStageBytes);
+          // the first CTA's barrier counts the bytes of both
+          const uint32_t bar = map_shared_rank(smem_u32(&full[stage]), 0);
+          if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * kStageBytes);
+          const int ma = it.m0 + rank * kHalf, nb = it.n0 + rank * kHalf;
           if (MODE != kProd) {
-            tma_load_2d(pa, &maps.a0, kb * kBK, it.m0, &full[stage]);
-            tma_load_2d(pb, &maps.b0, kb * kBK, a.v0 + it.n0, &full[stage]);
+            pair_load_2d(pa, &maps.a0, kb * kBK, ma, bar);
+            pair_load_2d(pb, &maps.b0, kb * kBK, a.v0 + nb, bar);
           } else if (it.kind == 0) {
-            tma_load_2d(pa, &maps.a0, kb * kBK, it.m0, &full[stage]);
+            pair_load_2d(pa, &maps.a0, kb * kBK, ma, bar);
 #pragma unroll
-            for (int j = 0; j < kBN / 64; ++j)
-              tma_load_2d(pb + j * kBox, &maps.b0, it.n0 + j * 64, a.v0 + kb * kBK, &full[stage]);
+            for (int j = 0; j < kHalf / 64; ++j)
+              pair_load_2d(pb + j * kBox, &maps.b0, nb + j * 64, a.v0 + kb * kBK, bar);
           } else {
 #pragma unroll
-            for (int j = 0; j < kBM / 64; ++j)
-              tma_load_2d(pa + j * kBox, &maps.a1, it.m0 + j * 64, kb * kBK, &full[stage]);
-#pragma unroll
-            for (int j = 0; j < kBN / 64; ++j)
-              tma_load_2d(pb + j * kBox, &maps.b1, it.n0 + j * 64, kb * kBK, &full[stage]);
+            for (int j = 0; j < kHalf / 64; ++j) {
+              pair_load_2d(pa + j * kBox, &maps.a1, ma + j * 64, kb * kBK, bar);
+              pair_load_2d(pb + j * kBox, &maps.b1, nb + j * 64, kb * kBK, bar);
+            }
           }
           ++issued;
           if (++stage == kStages) {
@@ -260,8 +301,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      if (!ok) {
-        // copies in flight land before the CTA may exit
+      if (!ok && rank == 0) {
+        // copies in flight land before the pair may exit
         for (int s = 0; s < kStages && s < issued; ++s) {
           const int fills = (issued - s + kStages - 1) / kStages;
           mbar_wait(&full[s], static_cast<uint32_t>((fills - 1) & 1), nullptr, 0);
@@ -269,13 +310,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
+    // ------------------------------------------------ MMA issuer, for both CTAs
+    if (lane == 0 && rank == 0) {
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
       const uint32_t base_a = smem_u32(sA), base_b = smem_u32(sB);
-      for (int w = blockIdx.x; w < total && ok; w += gridDim.x) {
+      for (int w = pair; w < total && ok; w += pairs) {
         const Item it = item_at<MODE>(a, rows, w);
         if (it.kb0 >= it.kb1) continue;
         if (!mbar_wait(&tempty[acc], acc_phase ^ 1, a.status, kErrAccumWait)) {
@@ -298,21 +339,21 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int k = 0; k < kBK / 16; ++k) {
             const uint64_t ad = mn_a ? sdesc_mn_sw128(pa + k * 2048, kBox, 1024) : sdesc_k_sw128(pa + k * 32);
             const uint64_t bd = mn_b ? sdesc_mn_sw128(pb + k * 2048, kBox, 1024) : sdesc_k_sw128(pb + k * 32);
-            tc_mma_bf16(d, ad, bd, idesc, (kb > it.kb0 || k > 0) ? 1u : 0u);
+            pair_mma(d, ad, bd, idesc, (kb > it.kb0 || k > 0) ? 1u : 0u);
           }
-          tc_commit(&empty[stage]);
+          pair_commit(&empty[stage]);
           if (++stage == kStages) {
             stage = 0;
             phase ^= 1;
           }
         }
         if (!ok) break;
-        tc_commit(&tfull[acc]);
+        pair_commit(&tfull[acc]);
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1;
       }
       // every issued MMA completes before TMEM is released
-      tc_commit(drain);
+      pair_commit(drain);
       mbar_wait(drain, 0, a.status, kErrMmaWait);
     }
   } else {
@@ -322,9 +363,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* out = sOut + quarter * 2 * kOutBytes;
     int acc = 0, staged = 0;
     uint32_t acc_phase = 0;
-    for (int w = blockIdx.x; w < total; w += gridDim.x) {
+    for (int w = pair; w < total; w += pairs) {
       const Item it = item_at<MODE>(a, rows, w);
-      const int m = it.m0 + quarter * 32 + lane;
+      const int m0 = it.m0 + rank * kHalf + quarter * 32;   // first row of this warp
+      const int m = m0 + lane;
       const bool empty_sum = it.kb0 >= it.kb1;
       if (empty_sum && !(MODE == kProd && it.kind == 1)) continue;
       // row inputs, fetched while the tile is still being multiplied
@@ -435,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
-            tma_store_2d(&maps.out0, box, it.n0 + c * 64, it.m0 + quarter * 32);
+            tma_store_2d(&maps.out0, box, it.n0 + c * 64, m0);
             bulk_commit();
           }
           ++staged;
@@ -456,7 +498,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
-            const int y = it.split * a.rpad + it.m0 + quarter * 32;
+            const int y = it.split * a.rpad + m0;
             if (a.first_piece)
               tma_store_2d(&maps.out0, box, it.n0 + c * 32, y);
             else
@@ -467,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       } else {
         // head gradient of the piece: complete, rounded once
-        const bool in_rows = a.v0 + it.m0 + quarter * 32 < a.V;
+        const bool in_rows = a.v0 + m0 < a.V;
         for (int c = 0; c < kBN / 64; ++c) {
           if (it.n0 + c * 64 >= a.H) break;
           uint8_t* box = out + (staged & 1) * kOutBytes;
@@ -493,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
           if (lane == 0) {
             // a group for every box, stored or not: the waits above count groups
-            if (in_rows) tma_store_2d(&maps.out1, box, it.n0 + c * 64, a.v0 + it.m0 + quarter * 32);
+            if (in_rows) tma_store_2d(&maps.out1, box, it.n0 + c * 64, a.v0 + m0);
             bulk_commit();
           }
           ++staged;
@@ -502,7 +544,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!empty_sum) {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&tempty[acc]);
+        if (lane == 0) remote_arrive(map_shared_rank(smem_u32(&tempty[acc]), 0));
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1;
       }
@@ -511,9 +553,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
+  cluster_sync();   // neither CTA leaves while the other may still signal its barriers
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 2 * kBN);
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * kBN) : "memory");
   }
 }
 
@@ -835,7 +878,7 @@ cudaError_t launch_gemm(const Maps& maps, const GemmArgs& a, int max_items, cuda
     if (e != cudaSuccess) return e;
     if (dev < 64) set[dev] = true;
   }
-  const int grid = std::max(1, std::min(max_items, device_sms()));
+  const int grid = 2 * std::max(1, std::min(max_items, device_sms() / 2));
   return launch_pdl(head_gemm_kernel<MODE>, dim3(grid), dim3(kThreads), kSmem, stream, maps, a);
 }
 
@@ -867,7 +910,7 @@ int head_loss_piece(int rpad, int V) {
 int head_loss_splits(int R, int H, int piece, int V) {
   const int tiles = ceil_div(R, kBM) * ceil_div(H, kBN);
   const int kb = ceil_div(std::min(piece, V), kBK);
-  const int want = std::max(1, std::min({device_sms() / std::max(1, tiles), kb / 4, 32}));
+  const int want = std::max(1, std::min({device_sms() / 2 / std::max(1, tiles), kb / 4, 32}));
   const int per = ceil_div(kb, want);
   return ceil_div(kb, per);
 }
@@ -886,8 +929,8 @@ cudaError_t head_loss_rows_launch(const HeadLossState& s, const HeadTargets& t, 
 
 cudaError_t head_loss_forward_launch(const HeadLossState& s, const HeadStatsScratch& p, cudaStream_t stream) {
   Maps maps{};
-  if (!map_bf16(&maps.a0, s.hc, s.rpad, s.H, s.H, kBK, kBM)) return cudaErrorInvalidValue;
-  if (!map_bf16(&maps.b0, s.w, s.V, s.H, s.ldw, kBK, kBN)) return cudaErrorInvalidValue;
+  if (!map_bf16(&maps.a0, s.hc, s.rpad, s.H, s.H, kBK, kHalf)) return cudaErrorInvalidValue;
+  if (!map_bf16(&maps.b0, s.w, s.V, s.H, s.ldw, kBK, kHalf)) return cudaErrorInvalidValue;
   GemmArgs a = base_args(s);
   a.v0 = 0;
   a.cols = s.V;
@@ -907,10 +950,10 @@ cudaError_t head_loss_backward_launch(const HeadLossState& s, const HeadGradArgs
   if (e != cudaSuccess) return e;
   Maps gm{}, pm{};
   const bool dh = g.dh != nullptr, dw = g.dw != nullptr;
-  if (!map_bf16(&gm.a0, s.hc, s.rpad, s.H, s.H, kBK, kBM) || !map_bf16(&gm.b0, s.w, s.V, s.H, s.ldw, kBK, kBN) ||
+  if (!map_bf16(&gm.a0, s.hc, s.rpad, s.H, s.H, kBK, kHalf) || !map_bf16(&gm.b0, s.w, s.V, s.H, s.ldw, kBK, kHalf) ||
       !map_bf16(&gm.out0, g.dl, s.rpad, g.piece, g.piece, 64, 32))
     return cudaErrorInvalidValue;
-  if (dh && (!map_bf16(&pm.a0, g.dl, s.rpad, g.piece, g.piece, kBK, kBM) ||
+  if (dh && (!map_bf16(&pm.a0, g.dl, s.rpad, g.piece, g.piece, kBK, kHalf) ||
              !map_bf16(&pm.b0, s.w, s.V, s.H, s.ldw, 64, kBK) ||
              !encode(&pm.out0, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, g.dh_part,
                      static_cast<long long>(g.splits) * s.rpad, s.H, s.H, 32, 32)))
