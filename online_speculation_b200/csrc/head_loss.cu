@@ -21,6 +21,10 @@
 //   outputs), and feed two products: dW of the piece is complete at once, dh adds up in fp32.
 //   Both read dl and their other operand in the layout they already have (MN-major
 //   shared-memory descriptors): nothing is transposed.
+// * Up to 256 rows take the products the other way around, vocabulary columns in the accumulator's
+//   lanes and rows in its columns.  A pass over few rows is the reading of the head, and a tile of
+//   256 lanes that holds 64 rows would spend four times the matrix instructions (and the clock that
+//   their power costs: 93 % tensor-pipe active at 1.5 GHz for 64 rows) on lanes that nobody looks at.
 #include "common.cuh"
 #include "head_loss.h"
 
@@ -34,14 +38,20 @@ constexpr int kBM = 256;                  // tile rows: 128 TMEM lanes in each C
 constexpr int kBN = 256;                  // tile columns: both CTAs hold all of them for their rows
 constexpr int kHalf = 128;                // rows of A, and of B, that one CTA stages
 constexpr int kBK = 64;                   // reduction elements a stage: one 128-byte swizzle row
-constexpr int kStages = 6;
-constexpr int kABytes = kHalf * kBK * 2;
-constexpr int kBBytes = kHalf * kBK * 2;
-constexpr int kStageBytes = kABytes + kBBytes;
+constexpr int kMaxStages = 12;
+constexpr int kRowBytes = kBK * 2;        // one staged row of either operand
 constexpr int kBox = 64 * 64 * 2;         // one MN-major box: 64 reduction rows of 64 elements
 constexpr int kOutBytes = 32 * 128;       // one warp's staged output box: 32 rows of 128 bytes
 constexpr int kThreads = 192;             // TMA warp, MMA warp, four epilogue warps
-constexpr int kSmem = 1024 + kStages * kStageBytes + 4 * 2 * kOutBytes + 256;
+constexpr int kOutTotal = 4 * 2 * kOutBytes;
+constexpr int kFewRows = 256;             // rows that fit the accumulator's columns
+// Per-row state of the passes with rows in columns, behind the output boxes: running maximum and sum and
+// plain sum (one set a warp), list cursors (one set a warp), coefficients, row numbers.
+constexpr int kStateMax = 0, kStateSum = kStateMax + 4 * kFewRows * 4, kStatePlain = kStateSum + 4 * kFewRows * 4,
+              kStateCursor = kStatePlain + 4 * kFewRows * 4, kStateCoef = kStateCursor + 4 * kFewRows * 8,
+              kStateRow = kStateCoef + kFewRows * 16, kStateBytes = kStateRow + kFewRows * 4;
+constexpr int kBarBytes = 256;            // barriers and the TMEM address
+constexpr int kSmemMost = 232448 - 1024;               // behind the alignment
 constexpr float kLog2e = 1.4426950408889634f;
 
 enum Mode { kStats = 0, kGrad = 1, kProd = 2 };
@@ -56,7 +66,11 @@ struct GemmArgs {
   const int* count;
   int H, V;
   int v0, cols;            // this piece: first vocabulary row, columns that exist
+  int bn;                  // rows in columns: how many columns, a multiple of 16
   int tiles_n;             // column tiles of the accumulator grid
+  int slot;                // rows in columns: vocabulary columns in the lanes of one CTA (statistics: a multiple of
+                           // 8, gradient: of 32)
+  int stages;              // of the ring
   int K;
   const int* row_of;
   const int* list_id;
@@ -67,10 +81,25 @@ struct GemmArgs {
   float2* part;
   float* part_sum;
   int part_tiles;
-  int rpad;
+  int rpad, piece;
   int do_dh, do_dw, splits, first_piece;
   int* status;
 };
+
+struct StageBytes {
+  int a, b;
+};
+
+// Shared memory of one stage: this CTA's part of either operand.
+__host__ __device__ inline StageBytes stage_bytes_of(int mode, bool few, const GemmArgs& a) {
+  if (few && mode != kProd) return {a.slot * kRowBytes, a.bn / 2 * kRowBytes};
+  if (few && !a.do_dw) return {kHalf * kRowBytes, (a.bn / 2 + 63) / 64 * kBox};
+  return {kHalf * kRowBytes, kHalf * kRowBytes};
+}
+
+__host__ __device__ inline int out_bytes_of(int mode, bool few) {
+  return mode == kStats ? (few ? kOutTotal / 2 : 0) : kOutTotal;
+}
 
 // One work item: an accumulator tile and its range of reduction blocks.
 struct Item {
@@ -80,48 +109,59 @@ struct Item {
   int split;
 };
 
-template <int MODE>
-__device__ __forceinline__ int item_count(const GemmArgs& a, int rows) {
-  const int tm = (rows + kBM - 1) / kBM;
-  if (MODE != kProd) return tm * a.tiles_n;
-  const int tv = (a.cols + kBM - 1) / kBM;
-  return (a.do_dh ? tm * a.tiles_n * a.splits : 0) + (a.do_dw ? tv * a.tiles_n : 0);
-}
-
-template <int MODE>
-__device__ __forceinline__ Item item_at(const GemmArgs& a, int rows, int w) {
-  Item it;
-  const int tm = (rows + kBM - 1) / kBM;
+// The i-th item of CTA pair `pair`; false behind its last.  FEW: rows in the accumulator's columns.
+template <int MODE, bool FEW>
+__device__ __forceinline__ bool item_at(const GemmArgs& a, int rows, int pair, int pairs, int i, Item& it) {
+  const int tm = (rows + kBM - 1) / kBM;    // row tiles
   it.split = 0;
+  it.kind = 0;
+  it.kb0 = 0;
+  it.n0 = 0;
   if (MODE != kProd) {
-    // rows fastest: the CTAs that run together read few head tiles, and the hidden rows stay in L2
-    it.kind = 0;
+    const int w = pair + i * pairs;
+    it.kb1 = (a.H + kBK - 1) / kBK;
+    if (FEW) {
+      it.m0 = w * 2 * a.slot;
+      return it.m0 < a.cols && rows > 0;
+    }
+    // rows fastest: the pairs that run together read few head tiles, and the hidden rows stay in L2
+    if (w >= tm * a.tiles_n) return false;
     it.m0 = (w % tm) * kBM;
     it.n0 = (w / tm) * kBN;
-    it.kb0 = 0;
-    it.kb1 = (a.H + kBK - 1) / kBK;
-    return it;
+    return true;
   }
-  const int nh = a.do_dh ? tm * a.tiles_n * a.splits : 0;
-  if (w < nh) {
-    const int kb = (a.cols + kBK - 1) / kBK, per = (kb + a.splits - 1) / a.splits;
-    const int per_split = tm * a.tiles_n;
-    it.kind = 0;
+  // The hidden gradient's items reduce over the piece, the head gradient's over the rows, and cost
+  // accordingly: the former go first, dealt around; the pairs that got one less take as many of the
+  // latter in its place as weigh the same, and the rest is dealt around.
+  const int kb = (a.cols + kBK - 1) / kBK, per = (kb + a.splits - 1) / a.splits, kbw = (rows + kBK - 1) / kBK;
+  const int per_split = FEW ? (rows > 0 ? a.tiles_n : 0) : tm * a.tiles_n;   // a.tiles_n tiles across the hidden width
+  const int nh = a.do_dh ? per_split * a.splits : 0;
+  const int nw = a.do_dw ? ((a.cols + kBM - 1) / kBM) * a.tiles_n : 0;
+  const int extra = nh % pairs, mine = nh / pairs + (pair < extra ? 1 : 0);
+  if (i < mine) {
+    const int w = pair + i * pairs, t = w % per_split;
     it.split = w / per_split;
-    const int t = w % per_split;
-    it.m0 = (t / a.tiles_n) * kBM;
-    it.n0 = (t % a.tiles_n) * kBN;
+    it.m0 = (FEW ? t : t / a.tiles_n) * kBM;
+    if (!FEW) it.n0 = (t % a.tiles_n) * kBN;
     it.kb0 = min(kb, it.split * per);
     it.kb1 = min(kb, it.kb0 + per);
-  } else {
-    const int t = w - nh;
-    it.kind = 1;
-    it.m0 = (t / a.tiles_n) * kBM;
-    it.n0 = (t % a.tiles_n) * kBN;
-    it.kb0 = 0;
-    it.kb1 = (rows + kBK - 1) / kBK;
+    return true;
   }
-  return it;
+  int j = i - mine, t;
+  const int late = extra > 0 ? pairs - extra : 0;   // pairs with one less
+  const int each = late > 0 && kbw > 0 ? min((per + kbw / 2) / kbw, nw / late) : 0;
+  if (late > 0 && pair >= extra && j < each) {
+    t = pair - extra + j * late;
+  } else {
+    if (late > 0 && pair >= extra) j -= each;
+    t = each * late + pair + j * pairs;
+  }
+  if (t >= nw) return false;
+  it.kind = 1;
+  it.m0 = (t / a.tiles_n) * kBM;
+  it.n0 = (t % a.tiles_n) * kBN;
+  it.kb1 = kbw;
+  return true;
 }
 
 // ------------------------------------------------------------- CTA pairs ----
@@ -213,17 +253,66 @@ struct ListCursor {
   }
 };
 
-template <int MODE>
+// Reduces 32 columns over the warp's lanes; lane j returns column j's.
+template <typename Op>
+__device__ __forceinline__ float reduce_columns(float (&x)[32], Op op) {
+  const int lane = threadIdx.x % 32;
+#pragma unroll
+  for (int n = 16; n > 0; n >>= 1) {
+    const bool up = (lane & n) != 0;
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const float send = up ? x[i] : x[i + n], keep = up ? x[i + n] : x[i];
+      x[i] = op(keep, __shfl_xor_sync(0xffffffffu, send, n));
+    }
+  }
+  return x[0];
+}
+
+// A warp's 32 x 32 block in shared memory (4 KB, lane = row), for the rare access to one element of
+// another lane's registers.
+__device__ __forceinline__ void spill_block(uint8_t* buf, const float (&x)[32]) {
+  const int lane = threadIdx.x % 32;
+#pragma unroll
+  for (int q = 0; q < 8; ++q)
+    *reinterpret_cast<float4*>(buf + swizzled(lane, q)) = make_float4(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]);
+  __syncwarp();
+}
+
+__device__ __forceinline__ void reload_block(const uint8_t* buf, float (&x)[32]) {
+  const int lane = threadIdx.x % 32;
+  __syncwarp();
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    const float4 v = *reinterpret_cast<const float4*>(buf + swizzled(lane, q));
+    x[4 * q] = v.x;
+    x[4 * q + 1] = v.y;
+    x[4 * q + 2] = v.z;
+    x[4 * q + 3] = v.w;
+  }
+  __syncwarp();
+}
+
+__device__ __forceinline__ float* block_at(uint8_t* buf, int row, int col) {
+  return reinterpret_cast<float*>(buf + swizzled(row, col >> 2) + (col & 3) * 4);
+}
+
+template <int MODE, bool FEW>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     head_gemm_kernel(const __grid_constant__ Maps maps, const GemmArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sA = smem;
-  uint8_t* sB = smem + kStages * kABytes;
-  uint8_t* sOut = smem + kStages * kStageBytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(sOut + 4 * 2 * kOutBytes);
-  uint64_t* empty = full + kStages;
-  uint64_t* tfull = empty + kStages;
+  // A stage is this CTA's part of the first operand, then of the second.  The matrix instruction takes 128
+  // lanes of the first whatever `slot` is: what it reads behind them (of the second) only reaches
+  // accumulator lanes that nobody looks at.
+  const StageBytes sb = stage_bytes_of(MODE, FEW, a);
+  const int stage_bytes = sb.a + sb.b;
+  const int stages = a.stages;
+  uint8_t* sOut = smem + stages * stage_bytes;
+  uint8_t* state = sOut + out_bytes_of(MODE, FEW);
+  uint64_t* full = reinterpret_cast<uint64_t*>(state + (FEW && MODE != kProd ? kStateBytes : 0));
+  uint64_t* empty = full + kMaxStages;
+  uint64_t* tfull = empty + kMaxStages;
   uint64_t* tempty = tfull + 2;
   uint64_t* drain = tempty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
@@ -232,7 +321,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int pair = blockIdx.x / 2, pairs = gridDim.x / 2;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < stages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
@@ -258,7 +347,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   pdl_trigger();
   pdl_wait();
   const int rows = *a.count;
-  const int total = item_count<MODE>(a, rows);
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
@@ -266,36 +354,55 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       int stage = 0, issued = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int w = pair; w < total && ok; w += pairs) {
-        const Item it = item_at<MODE>(a, rows, w);
+      Item it;
+      for (int i = 0; ok && item_at<MODE, FEW>(a, rows, pair, pairs, i, it); ++i) {
         for (int kb = it.kb0; kb < it.kb1; ++kb) {
           if (!mbar_wait(&empty[stage], phase ^ 1, a.status, kErrTmaWait)) {
             ok = false;
             break;
           }
-          uint8_t* pa = sA + stage * kABytes;
-          uint8_t* pb = sB + stage * kBBytes;
+          uint8_t* pa = smem + stage * stage_bytes;
+          uint8_t* pb = pa + sb.a;
           // the first CTA's barrier counts the bytes of both
           const uint32_t bar = map_shared_rank(smem_u32(&full[stage]), 0);
-          if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * kStageBytes);
-          const int ma = it.m0 + rank * kHalf, nb = it.n0 + rank * kHalf;
-          if (MODE != kProd) {
-            pair_load_2d(pa, &maps.a0, kb * kBK, ma, bar);
-            pair_load_2d(pb, &maps.b0, kb * kBK, a.v0 + nb, bar);
-          } else if (it.kind == 0) {
-            pair_load_2d(pa, &maps.a0, kb * kBK, ma, bar);
+          const int k0 = kb * kBK;
+          const bool hidden = MODE == kProd && it.kind == 0;
+          const int rows_box = (a.bn / 2 + 63) / 64;   // rows in columns: boxes of 64 rows
+          if (rank == 0) {
+            const int bytes = MODE != kProd ? stage_bytes
+                              : FEW && hidden ? kHalf * kRowBytes + rows_box * kBox
+                                              : 2 * kHalf * kRowBytes;
+            mbar_arrive_expect_tx(&full[stage], 2 * bytes);
+          }
+          if (FEW && MODE != kProd) {
+            pair_load_2d(pa, &maps.a0, k0, a.v0 + it.m0 + rank * a.slot, bar);
+            pair_load_2d(pb, &maps.b0, k0, rank * (a.bn / 2), bar);
+          } else if (FEW && hidden) {
 #pragma unroll
             for (int j = 0; j < kHalf / 64; ++j)
-              pair_load_2d(pb + j * kBox, &maps.b0, nb + j * 64, a.v0 + kb * kBK, bar);
+              pair_load_2d(pa + j * kBox, &maps.a0, it.m0 + rank * kHalf + j * 64, a.v0 + k0, bar);
+            for (int j = 0; j < rows_box; ++j)
+              pair_load_2d(pb + j * kBox, &maps.b0, rank * (a.bn / 2) + j * 64, k0, bar);
           } else {
+            const int ma = it.m0 + rank * kHalf, nb = it.n0 + rank * kHalf;
+            if (MODE != kProd) {
+              pair_load_2d(pa, &maps.a0, k0, ma, bar);
+              pair_load_2d(pb, &maps.b0, k0, a.v0 + nb, bar);
+            } else if (hidden) {
+              pair_load_2d(pa, &maps.a0, k0, ma, bar);
 #pragma unroll
-            for (int j = 0; j < kHalf / 64; ++j) {
-              pair_load_2d(pa + j * kBox, &maps.a1, ma + j * 64, kb * kBK, bar);
-              pair_load_2d(pb + j * kBox, &maps.b1, nb + j * 64, kb * kBK, bar);
+              for (int j = 0; j < kHalf / 64; ++j) pair_load_2d(pb + j * kBox, &maps.b0, nb + j * 64, a.v0 + k0, bar);
+            } else {
+              if (FEW) pair_load_2d(pa, &maps.a1, k0, ma, bar);
+#pragma unroll
+              for (int j = 0; j < kHalf / 64; ++j) {
+                if (!FEW) pair_load_2d(pa + j * kBox, &maps.a1, ma + j * 64, k0, bar);
+                pair_load_2d(pb + j * kBox, &maps.b1, nb + j * 64, k0, bar);
+              }
             }
           }
           ++issued;
-          if (++stage == kStages) {
+          if (++stage == stages) {
             stage = 0;
             phase ^= 1;
           }
@@ -303,8 +410,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       if (!ok && rank == 0) {
         // copies in flight land before the pair may exit
-        for (int s = 0; s < kStages && s < issued; ++s) {
-          const int fills = (issued - s + kStages - 1) / kStages;
+        for (int s = 0; s < stages && s < issued; ++s) {
+          const int fills = (issued - s + stages - 1) / stages;
           mbar_wait(&full[s], static_cast<uint32_t>((fills - 1) & 1), nullptr, 0);
         }
       }
@@ -315,9 +422,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
-      const uint32_t base_a = smem_u32(sA), base_b = smem_u32(sB);
-      for (int w = pair; w < total && ok; w += pairs) {
-        const Item it = item_at<MODE>(a, rows, w);
+      const uint32_t base = smem_u32(smem);
+      Item it;
+      for (int i = 0; ok && item_at<MODE, FEW>(a, rows, pair, pairs, i, it); ++i) {
         if (it.kb0 >= it.kb1) continue;
         if (!mbar_wait(&tempty[acc], acc_phase ^ 1, a.status, kErrAccumWait)) {
           ok = false;
@@ -325,16 +432,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         tc_fence_after();
         const uint32_t d = tmem + acc * kBN;
-        const bool mn_a = MODE == kProd && it.kind == 1, mn_b = MODE == kProd;
-        const uint32_t idesc =
-            idesc_bf16_f32(kBM, kBN) | (mn_a ? 1u << 15 : 0u) | (mn_b ? 1u << 16 : 0u);
+        const bool mn_a = MODE == kProd && (it.kind == (FEW ? 0 : 1)), mn_b = MODE == kProd;
+        const int columns = FEW && it.kind == 0 ? a.bn : kBN;
+        const uint32_t idesc = idesc_bf16_f32(kBM, columns) | (mn_a ? 1u << 15 : 0u) | (mn_b ? 1u << 16 : 0u);
         for (int kb = it.kb0; kb < it.kb1; ++kb) {
           if (!mbar_wait(&full[stage], phase, a.status, kErrMmaWait)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t pa = base_a + stage * kABytes, pb = base_b + stage * kBBytes;
+          const uint32_t pa = base + stage * stage_bytes, pb = pa + sb.a;
 #pragma unroll
           for (int k = 0; k < kBK / 16; ++k) {
             const uint64_t ad = mn_a ? sdesc_mn_sw128(pa + k * 2048, kBox, 1024) : sdesc_k_sw128(pa + k * 32);
@@ -342,7 +449,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             pair_mma(d, ad, bd, idesc, (kb > it.kb0 || k > 0) ? 1u : 0u);
           }
           pair_commit(&empty[stage]);
-          if (++stage == kStages) {
+          if (++stage == stages) {
             stage = 0;
             phase ^= 1;
           }
@@ -363,9 +470,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     uint8_t* out = sOut + quarter * 2 * kOutBytes;
     int acc = 0, staged = 0;
     uint32_t acc_phase = 0;
-    for (int w = pair; w < total; w += pairs) {
-      const Item it = item_at<MODE>(a, rows, w);
-      const int m0 = it.m0 + rank * kHalf + quarter * 32;   // first row of this warp
+    if (FEW && MODE != kProd) {
+      for (int t = threadIdx.x - 64; t < kFewRows; t += 128) {
+        const int o = t < rows ? a.row_of[t] : -1;
+        reinterpret_cast<int*>(state + kStateRow)[t] = o;
+        float4 c = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (MODE == kGrad && o >= 0) c = a.row_coef[t];
+        if (MODE == kStats) c.x = (o >= 0 && a.inv_temp != nullptr ? a.inv_temp[o] : 1.0f) * kLog2e;
+        reinterpret_cast<float4*>(state + kStateCoef)[t] = c;
+      }
+      if (MODE == kStats) {
+        for (int t = lane; t < kFewRows; t += 32) {
+          reinterpret_cast<float*>(state + kStateMax)[quarter * kFewRows + t] = -INFINITY;
+          reinterpret_cast<float*>(state + kStateSum)[quarter * kFewRows + t] = 0.0f;
+          reinterpret_cast<float*>(state + kStatePlain)[quarter * kFewRows + t] = 0.0f;
+        }
+      }
+      named_barrier(1, 128);
+    }
+    const int* row_no = reinterpret_cast<const int*>(state + kStateRow);
+    const float4* coef_of = reinterpret_cast<const float4*>(state + kStateCoef);
+    int2* cursors = reinterpret_cast<int2*>(state + kStateCursor) + quarter * kFewRows;
+    Item it;
+    for (int i = 0; item_at<MODE, FEW>(a, rows, pair, pairs, i, it); ++i) {
+      const int held = FEW && MODE != kProd ? a.slot : kHalf;
+      const int m0 = it.m0 + rank * held + quarter * 32;    // first tile row of this warp
       const int m = m0 + lane;
       const bool empty_sum = it.kb0 >= it.kb1;
       if (empty_sum && !(MODE == kProd && it.kind == 1)) continue;
@@ -375,7 +504,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       float c2 = kLog2e;
       float4 coef = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       bool live = false;
-      if (MODE != kProd) {
+      if (FEW && MODE != kProd) {
+        // every row's place in its list, for this warp's vocabulary columns
+        for (int t = lane; t < rows; t += 32) {
+          cur.seek(a.list_id + static_cast<long long>(row_no[t]) * a.K, a.K, a.v0 + m0);
+          cursors[t] = make_int2(cur.k, cur.next);
+        }
+        __syncwarp();
+      } else if (MODE != kProd) {
         live = m < rows;
         cur.k = 0;
         cur.K = 0;
@@ -395,23 +531,142 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       const uint32_t t_acc = tmem + lane_base + acc * kBN;
 
-      if (MODE == kStats) {
-        float mx = -INFINITY, sum = 0.0f, plain = 0.0f;
-        for (int c = 0; c < kBN / 32; ++c) {
-          float x[32];
-          tmem_ld32(t_acc + c * 32, x);
-          const int col = a.v0 + it.n0 + c * 32;       // vocabulary column of x[0]
-          if (col >= a.V) break;
-          if (a.part_sum != nullptr) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) plain += x[j];   // columns behind V are zero
+      if (FEW && MODE != kProd) {
+        // lanes are vocabulary columns, this thread's is `col`; chunks of 32 rows
+        const int first = a.v0 + m0;
+        const int stop = a.v0 + min(a.cols, it.m0 + (rank + 1) * held);   // behind this CTA's last column
+        const bool on = first + lane < stop;
+        float* maxes = reinterpret_cast<float*>(state + kStateMax) + quarter * kFewRows;
+        float* sums = reinterpret_cast<float*>(state + kStateSum) + quarter * kFewRows;
+        float* plains = reinterpret_cast<float*>(state + kStatePlain) + quarter * kFewRows;
+        // Runs `use(block)` for rows whose list has a column here, on the block in shared memory.
+        auto listed = [&](float (&x)[32], int t, uint8_t* buf, auto use) {
+          int2 c = t < rows ? cursors[t] : make_int2(0, INT_MAX);
+          const int end = min(first + 32, stop);
+          if (!__any_sync(0xffffffffu, c.y < end)) return;
+          spill_block(buf, x);
+          const long long base = t < rows ? static_cast<long long>(row_no[t]) * a.K : 0;
+          while (c.y < end) {
+            use(block_at(buf, c.y - first, lane), base + c.x);
+            ++c.x;
+            c.y = c.x < a.K ? a.list_id[base + c.x] : INT_MAX;
           }
-          if (col + 32 > a.V) {
+          reload_block(buf, x);
+        };
+        const int chunks = MODE == kStats ? (rows + 31) / 32 : 2 * ((rows + 63) / 64);
+        for (int c = 0; c < chunks && first < stop; ++c) {
+          const int t0 = c * 32, t = t0 + lane;
+          float x[32];
+          tmem_ld32(t_acc + t0, x);
+          if (MODE == kStats) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-              if (col + j >= a.V) x[j] = -INFINITY;
+              if (!on) x[j] = -INFINITY;
+            if (a.part_sum != nullptr) {
+              float y[32];
+#pragma unroll
+              for (int j = 0; j < 32; ++j) y[j] = on ? x[j] : 0.0f;
+              const float p = reduce_columns(y, [](float u, float v) { return u + v; });
+              plains[t] += p;
+            }
+            listed(x, t, sOut + quarter * kOutBytes, [&](float* at, long long k) {
+              a.list_logit[k] = *at;
+              *at = -INFINITY;
+            });
+            float y[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) y[j] = x[j];
+            const float top = reduce_columns(y, [](float u, float v) { return fmaxf(u, v); });
+            const float before = maxes[t], now = fmaxf(before, top);
+            const float kept = before == -INFINITY ? 0.0f : ex2((before - now) * coef_of[t].x);
+            maxes[t] = now;
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const float ref = maxes[t0 + j];
+              y[j] = ex2((x[j] - (ref == -INFINITY ? 0.0f : ref)) * coef_of[t0 + j].x);
+            }
+            const float s = reduce_columns(y, [](float u, float v) { return u + v; });
+            sums[t] = sums[t] * kept + s;
+            __syncwarp();
+          } else {
+            uint8_t* box = out + (staged & 1) * kOutBytes;
+            if ((c & 1) == 0) {
+              if (lane == 0) bulk_wait_read<1>();
+              __syncwarp();
+            }
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const float4 k = coef_of[t0 + j];
+              x[j] = k.z * ex2(fmaf(x[j], k.x, -k.y)) - k.w;
+            }
+            // the other box, once its store has read it, holds the block
+            int2 peek = t < rows ? cursors[t] : make_int2(0, INT_MAX);
+            if (__any_sync(0xffffffffu, peek.y < min(first + 32, stop))) {
+              if (lane == 0) bulk_wait_read<0>();
+              __syncwarp();
+              listed(x, t, out + ((staged + 1) & 1) * kOutBytes,
+                     [&](float* at, long long k) { *at = a.list_grad[k]; });
+            }
+            if (t0 + 32 > rows) {
+              // columns behind the rows hold what an earlier tile left
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (t0 + j >= rows) x[j] = 0.0f;
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const uint4 v = make_uint4(pack2(x[8 * q], x[8 * q + 1]), pack2(x[8 * q + 2], x[8 * q + 3]),
+                                         pack2(x[8 * q + 4], x[8 * q + 5]), pack2(x[8 * q + 6], x[8 * q + 7]));
+              *reinterpret_cast<uint4*>(box + swizzled(lane, (c & 1) * 4 + q)) = on ? v : make_uint4(0, 0, 0, 0);
+            }
+            if (c & 1) {
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                tma_store_2d(&maps.out0, box, (c >> 1) * 64, m0);
+                bulk_commit();
+              }
+              ++staged;
+            }
           }
-          while (cur.next < col + 32) {
+        }
+        if (MODE == kGrad && first >= stop && quarter * 32 < held && m0 < a.piece) {
+          // behind the vocabulary, but inside a block that the hidden gradient's product reads: zeros
+          for (int c = 0; c < (rows + 63) / 64; ++c) {
+            uint8_t* box = out + (staged & 1) * kOutBytes;
+            if (lane == 0) bulk_wait_read<1>();
+            __syncwarp();
+#pragma unroll
+            for (int q = 0; q < 8; ++q) *reinterpret_cast<uint4*>(box + swizzled(lane, q)) = make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&maps.out0, box, c * 64, m0);
+              bulk_commit();
+            }
+            ++staged;
+          }
+        }
+      } else if (MODE == kStats) {
+        float mx = -INFINITY, sum = 0.0f, plain = 0.0f;
+        const int end = min(a.V, it.n0 + kBN);         // behind the tile's last column
+        for (int c = 0; c < kBN / 32; ++c) {
+          const int col = it.n0 + c * 32;              // vocabulary column of x[0]
+          if (col >= end || m0 >= rows) break;
+          float x[32];
+          tmem_ld32(t_acc + c * 32, x);
+          if (col + 32 > end) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              if (col + j < end) plain += x[j];
+              else x[j] = -INFINITY;
+            }
+          } else if (a.part_sum != nullptr) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) plain += x[j];
+          }
+          while (cur.next < min(col + 32, end)) {
             const int at = cur.next - col;
             float v = 0.0f;
 #pragma unroll
@@ -482,6 +737,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           }
           ++staged;
         }
+      } else if (FEW && it.kind == 0) {
+        // hidden gradient with hidden columns in the lanes: turned around on the way into the box
+        for (int c = 0; c < (rows + 31) / 32 && m0 < a.H; ++c) {
+          float x[32];
+          tmem_ld32(t_acc + c * 32, x);
+          uint8_t* box = out + (staged & 1) * kOutBytes;
+          if (lane == 0) bulk_wait_read<1>();
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) *block_at(box, j, lane) = x[j];
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            const int y = it.split * a.rpad + c * 32;
+            if (a.first_piece)
+              tma_store_2d(&maps.out0, box, m0, y);
+            else
+              tma_add_2d(&maps.out0, box, m0, y);
+            bulk_commit();
+          }
+          ++staged;
+        }
       } else if (it.kind == 0) {
         // hidden gradient: fp32, added to what earlier pieces left
         for (int c = 0; c < kBN / 32; ++c) {
@@ -547,6 +824,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (lane == 0) remote_arrive(map_shared_rank(smem_u32(&tempty[acc]), 0));
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1;
+      }
+    }
+    if (FEW && MODE == kStats) {
+      const int column = blockIdx.x * 4 + quarter;
+      for (int t = lane; t < rows; t += 32) {
+        const long long p = static_cast<long long>(t) * a.part_tiles + column;
+        a.part[p] = make_float2(reinterpret_cast<float*>(state + kStateMax)[quarter * kFewRows + t],
+                                reinterpret_cast<float*>(state + kStateSum)[quarter * kFewRows + t]);
+        if (a.part_sum != nullptr) a.part_sum[p] = reinterpret_cast<float*>(state + kStatePlain)[quarter * kFewRows + t];
       }
     }
     if (lane == 0) bulk_wait_all();
@@ -867,19 +1153,46 @@ int device_sms() {
   return cached[dev];
 }
 
-template <int MODE>
-cudaError_t launch_gemm(const Maps& maps, const GemmArgs& a, int max_items, cudaStream_t stream) {
+int ceil_div(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
+
+// CTA pairs of a launch.
+int pairs_for(int items) { return std::max(1, std::min(items, device_sms() / 2)); }
+
+bool few_rows(int R) { return R <= kFewRows; }
+
+// Rows in columns: how many vocabulary columns one CTA's lanes hold, a multiple of `step`.  As many tiles as
+// fill the rounds: with 152064 columns on 74 pairs, 256 a tile make 594 tiles, two more than eight
+// rounds; 240 make nine nearly full ones.
+int lane_slot(int cols, int step) {
+  const int pairs = device_sms() / 2;
+  int best = kHalf;
+  long long cost = LLONG_MAX;
+  for (int w = kHalf; w >= 96; w -= step) {
+    const long long c = static_cast<long long>(ceil_div(ceil_div(cols, 2 * w), pairs)) * (w + 4);
+    if (c < cost) {
+      cost = c;
+      best = w;
+    }
+  }
+  return best;
+}
+
+template <int MODE, bool FEW>
+cudaError_t launch_gemm(const Maps& maps, GemmArgs a, int max_items, cudaStream_t stream) {
   static bool set[64] = {false};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev >= 64 || !set[dev]) {
-    e = cudaFuncSetAttribute(head_gemm_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    e = cudaFuncSetAttribute(head_gemm_kernel<MODE, FEW>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost + 1024);
     if (e != cudaSuccess) return e;
     if (dev < 64) set[dev] = true;
   }
-  const int grid = 2 * std::max(1, std::min(max_items, device_sms() / 2));
-  return launch_pdl(head_gemm_kernel<MODE>, dim3(grid), dim3(kThreads), kSmem, stream, maps, a);
+  const int rest = out_bytes_of(MODE, FEW) + (FEW && MODE != kProd ? kStateBytes : 0) + kBarBytes;
+  const StageBytes sb = stage_bytes_of(MODE, FEW, a);
+  a.stages = std::min(kMaxStages, (kSmemMost - rest) / (sb.a + sb.b));
+  const int smem = 1024 + a.stages * (sb.a + sb.b) + rest;
+  return launch_pdl(head_gemm_kernel<MODE, FEW>, dim3(2 * pairs_for(max_items)), dim3(kThreads), smem, stream, maps, a);
 }
 
 GemmArgs base_args(const HeadLossState& s) {
@@ -891,28 +1204,51 @@ GemmArgs base_args(const HeadLossState& s) {
   a.row_of = s.row_of;
   a.list_id = s.list_id;
   a.rpad = s.rpad;
+  a.slot = kHalf;
+  a.bn = few_rows(s.R) ? ceil_div(s.R, 16) * 16 : kBN;
   a.status = s.status;
   return a;
 }
 
-int ceil_div(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
-
 }  // namespace
 
-int head_loss_vocab_tiles(int V) { return ceil_div(V, kBN); }
+// Partial statistics per row: one a warp of the launch, or one a tile of columns.
+int head_loss_vocab_tiles(int R, int V) {
+  return few_rows(R) ? 8 * pairs_for(ceil_div(V, 2 * lane_slot(V, 8))) : ceil_div(V, kBN);
+}
 
-int head_loss_piece(int rpad, int V) {
-  long long piece = (128ll << 20) / (2ll * rpad) / kBN * kBN;
+// Row pitch or row count of the logits' gradient: [piece][few rows] or [rows][piece].
+int head_loss_grad_rows(int R) { return few_rows(R) ? ceil_div(R, 64) * 64 : ceil_div(R, kHeadRowPad) * kHeadRowPad; }
+
+// Columns of the logits that the backward pass works on at a time.  Their gradient takes two bytes a row and
+// column: 256 MB of it, so that a pass over a piece is long against the ends of its two launches.
+int head_loss_piece(int R, int V) {
+  long long piece = (256ll << 20) / (2ll * head_loss_grad_rows(R)) / kBN * kBN;
   piece = std::max<long long>(piece, 4096);
   return static_cast<int>(std::min<long long>(piece, static_cast<long long>(ceil_div(V, kBN)) * kBN));
 }
 
-int head_loss_splits(int R, int H, int piece, int V) {
-  const int tiles = ceil_div(R, kBM) * ceil_div(H, kBN);
-  const int kb = ceil_div(std::min(piece, V), kBK);
-  const int want = std::max(1, std::min({device_sms() / 2 / std::max(1, tiles), kb / 4, 32}));
-  const int per = ceil_div(kb, want);
-  return ceil_div(kb, per);
+// Parts of the hidden gradient's reduction over a piece.  Next to the head gradient's items, which fill
+// the pairs that it leaves idle, as few as keep one part from being longer than a pair's share of
+// everything; alone, as many as give every pair the same work.
+int head_loss_splits(int R, int H, int piece, int V, bool with_dw) {
+  const int pairs = device_sms() / 2, cols = std::min(piece, V), kb = ceil_div(cols, kBK);
+  const long long tiles = static_cast<long long>(few_rows(R) ? 1 : ceil_div(R, kBM)) * ceil_div(H, kBN);
+  const long long other = static_cast<long long>(ceil_div(cols, kBM)) * ceil_div(H, kBN) * ceil_div(R, kBK);
+  int best = 1;
+  long long cost = LLONG_MAX;
+  for (int want = 1; want <= 16 && want * 4 <= std::max(kb, 4); ++want) {
+    if (want > 1 && tiles >= 2 * pairs) break;          // enough tiles as they are
+    const int per = ceil_div(kb, want), splits = ceil_div(kb, per);
+    if (with_dw && per <= (tiles * kb + other) / pairs) return splits;
+    // a tile's end and its partial sums weigh about four blocks
+    const long long c = static_cast<long long>(ceil_div(tiles * splits, pairs)) * (per + 4);
+    if (c < cost) {
+      cost = c;
+      best = splits;
+    }
+  }
+  return best;
 }
 
 cudaError_t head_loss_rows_launch(const HeadLossState& s, const HeadTargets& t, cudaStream_t stream) {
@@ -929,8 +1265,7 @@ cudaError_t head_loss_rows_launch(const HeadLossState& s, const HeadTargets& t, 
 
 cudaError_t head_loss_forward_launch(const HeadLossState& s, const HeadStatsScratch& p, cudaStream_t stream) {
   Maps maps{};
-  if (!map_bf16(&maps.a0, s.hc, s.rpad, s.H, s.H, kBK, kHalf)) return cudaErrorInvalidValue;
-  if (!map_bf16(&maps.b0, s.w, s.V, s.H, s.ldw, kBK, kHalf)) return cudaErrorInvalidValue;
+  const bool few = few_rows(s.R);
   GemmArgs a = base_args(s);
   a.v0 = 0;
   a.cols = s.V;
@@ -940,7 +1275,18 @@ cudaError_t head_loss_forward_launch(const HeadLossState& s, const HeadStatsScra
   a.part = p.part;
   a.part_sum = p.part_sum;
   a.part_tiles = p.tiles;
-  cudaError_t e = launch_gemm<kStats>(maps, a, ceil_div(s.R, kBM) * a.tiles_n, stream);
+  cudaError_t e;
+  if (few) {
+    a.slot = lane_slot(s.V, 8);
+    if (!map_bf16(&maps.a0, s.w, s.V, s.H, s.ldw, kBK, a.slot) ||
+        !map_bf16(&maps.b0, s.hc, s.rpad, s.H, s.H, kBK, a.bn / 2))
+      return cudaErrorInvalidValue;
+    e = launch_gemm<kStats, true>(maps, a, ceil_div(s.V, 2 * a.slot), stream);
+  } else {
+    if (!map_bf16(&maps.a0, s.hc, s.rpad, s.H, s.H, kBK, kHalf) || !map_bf16(&maps.b0, s.w, s.V, s.H, s.ldw, kBK, kHalf))
+      return cudaErrorInvalidValue;
+    e = launch_gemm<kStats, false>(maps, a, ceil_div(s.R, kBM) * a.tiles_n, stream);
+  }
   if (e != cudaSuccess) return e;
   return launch_pdl(finish_rows_kernel, dim3(ceil_div(s.R, 4)), dim3(128), 0, stream, s, p);
 }
@@ -949,36 +1295,55 @@ cudaError_t head_loss_backward_launch(const HeadLossState& s, const HeadGradArgs
   cudaError_t e = launch_pdl(grad_rows_kernel, dim3(ceil_div(s.rpad, 4)), dim3(128), 0, stream, s, g);
   if (e != cudaSuccess) return e;
   Maps gm{}, pm{};
-  const bool dh = g.dh != nullptr, dw = g.dw != nullptr;
-  if (!map_bf16(&gm.a0, s.hc, s.rpad, s.H, s.H, kBK, kHalf) || !map_bf16(&gm.b0, s.w, s.V, s.H, s.ldw, kBK, kHalf) ||
-      !map_bf16(&gm.out0, g.dl, s.rpad, g.piece, g.piece, 64, 32))
-    return cudaErrorInvalidValue;
-  if (dh && (!map_bf16(&pm.a0, g.dl, s.rpad, g.piece, g.piece, kBK, kHalf) ||
-             !map_bf16(&pm.b0, s.w, s.V, s.H, s.ldw, 64, kBK) ||
-             !encode(&pm.out0, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, g.dh_part,
-                     static_cast<long long>(g.splits) * s.rpad, s.H, s.H, 32, 32)))
-    return cudaErrorInvalidValue;
-  if (dw && (!map_bf16(&pm.a1, g.dl, s.rpad, g.piece, g.piece, 64, kBK) ||
-             !map_bf16(&pm.b1, s.hc, s.rpad, s.H, s.H, 64, kBK) ||
-             !map_bf16(&pm.out1, g.dw, s.V, s.H, s.H, 64, 32)))
-    return cudaErrorInvalidValue;
+  const bool dh = g.dh != nullptr, dw = g.dw != nullptr, few = few_rows(s.R);
+  GemmArgs base = base_args(s);
+  base.piece = g.piece;
+  base.list_grad = g.list_grad;
+  base.row_coef = g.row_coef;
+  base.do_dh = dh;
+  base.do_dw = dw;
+  base.splits = g.splits;
+  const int slot = lane_slot(std::min(g.piece, s.V), 32), pitch = head_loss_grad_rows(s.R);
+  bool ok = true;
+  if (few) {
+    ok = map_bf16(&gm.a0, s.w, s.V, s.H, s.ldw, kBK, slot) && map_bf16(&gm.b0, s.hc, s.rpad, s.H, s.H, kBK, base.bn / 2) &&
+         map_bf16(&gm.out0, g.dl, g.piece, pitch, pitch, 64, 32);
+    if (dh)
+      ok = ok && map_bf16(&pm.a0, s.w, s.V, s.H, s.ldw, 64, kBK) &&
+           map_bf16(&pm.b0, g.dl, g.piece, pitch, pitch, 64, kBK);
+    if (dw) ok = ok && map_bf16(&pm.a1, g.dl, g.piece, pitch, pitch, kBK, kHalf);
+  } else {
+    ok = map_bf16(&gm.a0, s.hc, s.rpad, s.H, s.H, kBK, kHalf) && map_bf16(&gm.b0, s.w, s.V, s.H, s.ldw, kBK, kHalf) &&
+         map_bf16(&gm.out0, g.dl, s.rpad, g.piece, g.piece, 64, 32);
+    if (dh)
+      ok = ok && map_bf16(&pm.a0, g.dl, s.rpad, g.piece, g.piece, kBK, kHalf) &&
+           map_bf16(&pm.b0, s.w, s.V, s.H, s.ldw, 64, kBK);
+    if (dw) ok = ok && map_bf16(&pm.a1, g.dl, s.rpad, g.piece, g.piece, 64, kBK);
+  }
+  if (dh)
+    ok = ok && encode(&pm.out0, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, g.dh_part, static_cast<long long>(g.splits) * s.rpad,
+                      s.H, s.H, 32, 32);
+  if (dw)
+    ok = ok && map_bf16(&pm.b1, s.hc, s.rpad, s.H, s.H, 64, kBK) && map_bf16(&pm.out1, g.dw, s.V, s.H, s.H, 64, 32);
+  if (!ok) return cudaErrorInvalidValue;
   for (int v0 = 0; v0 < s.V; v0 += g.piece) {
-    GemmArgs a = base_args(s);
+    GemmArgs a = base;
     a.v0 = v0;
     a.cols = std::min(g.piece, s.V - v0);
-    a.tiles_n = ceil_div(a.cols, kBN);
-    a.list_grad = g.list_grad;
-    a.row_coef = g.row_coef;
-    e = launch_gemm<kGrad>(gm, a, ceil_div(s.R, kBM) * a.tiles_n, stream);
+    if (few) {
+      a.slot = slot;
+      e = launch_gemm<kGrad, true>(gm, a, ceil_div(a.cols, 2 * slot), stream);
+      a.slot = kHalf;
+    } else {
+      a.tiles_n = ceil_div(a.cols, kBN);
+      e = launch_gemm<kGrad, false>(gm, a, ceil_div(s.R, kBM) * a.tiles_n, stream);
+    }
     if (e != cudaSuccess) return e;
     a.tiles_n = ceil_div(s.H, kBN);
-    a.do_dh = dh;
-    a.do_dw = dw;
-    a.splits = g.splits;
     a.first_piece = v0 == 0;
-    const int items = (dh ? ceil_div(s.R, kBM) * a.tiles_n * g.splits : 0) +
+    const int items = (dh ? (few ? 1 : ceil_div(s.R, kBM)) * a.tiles_n * g.splits : 0) +
                       (dw ? ceil_div(a.cols, kBM) * a.tiles_n : 0);
-    e = launch_gemm<kProd>(pm, a, items, stream);
+    e = few ? launch_gemm<kProd, true>(pm, a, items, stream) : launch_gemm<kProd, false>(pm, a, items, stream);
     if (e != cudaSuccess) return e;
   }
   if (dh) return launch_pdl(hidden_grad_kernel, dim3(s.R), dim3(128), 0, stream, s, g);

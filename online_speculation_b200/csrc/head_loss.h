@@ -48,7 +48,7 @@ struct HeadTargets {
 };
 
 struct HeadStatsScratch {
-  float2* part;                // [rpad, tiles] max and sum exp of every vocabulary tile
+  float2* part;                // [rpad, tiles] max and sum exp of every vocabulary tile, or of every warp's share
   float* part_sum;             // [rpad, tiles] sum of logits (smoothing > 0) or null
   int tiles;
 };
@@ -58,7 +58,7 @@ struct HeadGradArgs {
   const float* g;              // [R] upstream gradient
   float4* row_coef;            // [rpad]
   float* list_grad;            // [R, K]
-  __nv_bfloat16* dl;           // [rpad, piece] gradient of one piece of the logits
+  __nv_bfloat16* dl;           // [rpad, piece] gradient of one piece of the logits, or [piece, few rows]
   int piece;                   // vocabulary columns a piece (multiple of 256)
   float* dh_part;              // [splits, rpad, H] or null
   int splits;
@@ -66,9 +66,10 @@ struct HeadGradArgs {
   __nv_bfloat16* dw;           // [V, H] contiguous or null
 };
 
-int head_loss_vocab_tiles(int V);                       // tiles of the statistics scratch
-int head_loss_piece(int rpad, int V);                   // default backward piece
-int head_loss_splits(int R, int H, int piece, int V);   // splits of the hidden gradient's reduction
+int head_loss_vocab_tiles(int R, int V);                // tiles of the statistics scratch
+int head_loss_grad_rows(int R);                         // rows (or row pitch) of the logits' gradient
+int head_loss_piece(int R, int V);                      // default backward piece
+int head_loss_splits(int R, int H, int piece, int V, bool with_dw);   // parts of the hidden gradient's reduction
 
 cudaError_t head_loss_rows_launch(const HeadLossState& s, const HeadTargets& t, cudaStream_t stream);
 cudaError_t head_loss_forward_launch(const HeadLossState& s, const HeadStatsScratch& p, cudaStream_t stream);

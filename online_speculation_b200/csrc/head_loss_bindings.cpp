@@ -132,7 +132,7 @@ std::tuple<Tensor, Tensor> head_loss_forward(Tensor h, Tensor weight, Tensor ids
     }
   }
   osb::HeadStatsScratch p{};
-  p.tiles = osb::head_loss_vocab_tiles(s.V);
+  p.tiles = osb::head_loss_vocab_tiles(s.R, s.V);
   const long long parts = static_cast<long long>(s.rpad) * p.tiles;
   Carve size{nullptr};
   size.take<float2>(parts);
@@ -170,9 +170,9 @@ std::tuple<OptTensor, OptTensor> head_loss_backward(Tensor saved, Tensor weight,
     TORCH_CHECK(piece % 256 == 0, "pieces are multiples of 256 columns");
     a.piece = static_cast<int>(std::min<int64_t>(piece, (V + 255) / 256 * 256));
   } else {
-    a.piece = osb::head_loss_piece(s.rpad, s.V);
+    a.piece = osb::head_loss_piece(s.R, s.V);
   }
-  a.splits = need_dh ? osb::head_loss_splits(s.R, s.H, a.piece, s.V) : 1;
+  a.splits = need_dh ? osb::head_loss_splits(s.R, s.H, a.piece, s.V, need_dw) : 1;
   const auto opts = weight.options();
   OptTensor dh, dw;
   if (need_dh) {
@@ -183,7 +183,7 @@ std::tuple<OptTensor, OptTensor> head_loss_backward(Tensor saved, Tensor weight,
     dw = torch::empty({V, H}, opts);
     a.dw = reinterpret_cast<__nv_bfloat16*>(dw->data_ptr());
   }
-  const long long dl = static_cast<long long>(s.rpad) * a.piece;
+  const long long dl = static_cast<long long>(osb::head_loss_grad_rows(s.R)) * a.piece;
   const long long parts = need_dh ? static_cast<long long>(a.splits) * s.rpad * H : 0;
   Carve size{nullptr};
   size.take<__nv_bfloat16>(dl);

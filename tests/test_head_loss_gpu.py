@@ -18,7 +18,7 @@ def _grads(loss, h, w, g):
 
 # rows, hidden, vocabulary: single rows and columns, one past a tile, odd, several tiles of each kind
 SHAPES = [(1, 8, 1), (1, 64, 500), (2, 72, 257), (33, 512, 2048), (129, 136, 777), (300, 264, 1025), (257, 64, 20001),
-          (64, 1536, 5000)]
+          (64, 1536, 5000), (256, 520, 20011), (177, 1000, 40000), (512, 136, 513)]
 
 
 @pytest.mark.parametrize("rows,hidden,vocab", SHAPES)
