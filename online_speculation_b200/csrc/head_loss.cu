@@ -77,6 +77,8 @@ struct GemmArgs {
   float* list_logit;       // stats: written
   const float* list_grad;  // grad: read
   const float4* row_coef;  // grad
+  HeadLossState s;         // rows in columns, grad: coefficients and listed values are formed on the spot
+  const float* g;
   const float* inv_temp;   // stats
   float2* part;
   float* part_sum;
@@ -252,6 +254,29 @@ struct ListCursor {
     next = k < K ? ids[k] : INT_MAX;
   }
 };
+
+// A row's coefficients of the logits' gradient: {it log2 e, lse log2 e, A, C} of A exp(it l - lse) - C.
+__device__ __forceinline__ float4 row_coefficients(const HeadLossState& s, const float* g, int r) {
+  const float4 st = s.row_stat[r];
+  const float it = s.inv_temp != nullptr ? s.inv_temp[r] : 1.0f;
+  const float up = g[r] * it;
+  const float flat = s.divergence ? 0.0f : s.smoothing / static_cast<float>(s.V);
+  return make_float4(it * kLog2e, st.x * kLog2e, up * st.z, up * flat);
+}
+
+// The gradient of the listed logit `at` of row r.
+__device__ __forceinline__ float listed_gradient(const HeadLossState& s, const float* g, int r, long long at) {
+  const float4 st = s.row_stat[r];
+  const float it = s.inv_temp != nullptr ? s.inv_temp[r] : 1.0f;
+  float v;
+  if (s.divergence) {
+    v = expf(s.list_logit[at] * it - st.x) - s.list_mass[at];
+  } else {
+    // a p - 1 with p - 1 = -(mass of the rest): no cancellation in sure rows
+    v = (st.z - 1.0f) * (1.0f - st.y) - st.y + s.smoothing - s.smoothing / static_cast<float>(s.V);
+  }
+  return g[r] * it * v;
+}
 
 // Reduces 32 columns over the warp's lanes; lane j returns column j's.
 template <typename Op>
@@ -475,7 +500,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const int o = t < rows ? a.row_of[t] : -1;
         reinterpret_cast<int*>(state + kStateRow)[t] = o;
         float4 c = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (MODE == kGrad && o >= 0) c = a.row_coef[t];
+        if (MODE == kGrad && o >= 0) c = row_coefficients(a.s, a.g, o);
         if (MODE == kStats) c.x = (o >= 0 && a.inv_temp != nullptr ? a.inv_temp[o] : 1.0f) * kLog2e;
         reinterpret_cast<float4*>(state + kStateCoef)[t] = c;
       }
@@ -606,7 +631,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
               if (lane == 0) bulk_wait_read<0>();
               __syncwarp();
               listed(x, t, out + ((staged + 1) & 1) * kOutBytes,
-                     [&](float* at, long long k) { *at = a.list_grad[k]; });
+                     [&](float* at, long long k) { *at = listed_gradient(a.s, a.g, row_no[t], k); });
             }
             if (t0 + 32 > rows) {
               // columns behind the rows hold what an earlier tile left
@@ -904,7 +929,8 @@ __global__ void __launch_bounds__(128) teacher_rows_kernel(const HeadLossState s
   for (int k = lane; k < K; k += 32) {
     const int v = id[k];
     bool first = v != INT_MAX;
-    for (int j = 0; j < k && first; ++j) first = id[j] != v;
+#pragma unroll 8
+    for (int j = 0; j < K; ++j) first = first && !(id[j] == v && j < k);
     key[k] = first ? v : INT_MAX;
   }
   __syncwarp();
@@ -914,11 +940,16 @@ __global__ void __launch_bounds__(128) teacher_rows_kernel(const HeadLossState s
     const int v = key[k];
     if (v == INT_MAX) continue;
     int at = 0;
-    double m = mass[k];
+    int twins = 0;
+#pragma unroll 8
     for (int j = 0; j < K; ++j) {
       at += key[j] < v;
-      if (j > k && id[j] == v) m += mass[j];
+      twins += id[j] == v;
     }
+    double m = mass[k];
+    if (twins > 1)
+      for (int j = k + 1; j < K; ++j)
+        if (id[j] == v) m += mass[j];
     s.list_id[base + at] = v;
     s.list_mass[base + at] = static_cast<float>(m * inv);
   }
@@ -975,6 +1006,58 @@ __global__ void __launch_bounds__(1024) compact_rows_kernel(const HeadLossState 
   if (threadIdx.x == 0) *s.count = n;
 }
 
+// Both at once for few rows: every block counts the rows before its own.
+__global__ void __launch_bounds__(128) few_rows_kernel(const HeadLossState s, const HeadTargets t) {
+  __shared__ int before_of[4], total_of[4];
+  pdl_trigger();
+  pdl_wait();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, b = blockIdx.x;
+  auto counts = [&](int r) {
+    if (r >= s.R) return false;
+    if (s.divergence) return t.active[r] != 0;
+    const long long v = load_id(t.ids, t.ids_i64, r);
+    return v != t.ignore_index && v >= 0 && v < s.V;
+  };
+  int before = 0, total = 0;
+  for (int r0 = warp * 32; r0 < kFewRows; r0 += 128) {
+    const unsigned on = __ballot_sync(0xffffffffu, counts(r0 + lane));
+    total += __popc(on);
+    before += r0 + 32 <= b ? __popc(on) : r0 < b ? __popc(on & ((1u << (b - r0)) - 1u)) : 0;
+  }
+  if (lane == 0) {
+    before_of[warp] = before;
+    total_of[warp] = total;
+  }
+  __syncthreads();
+  before = before_of[0] + before_of[1] + before_of[2] + before_of[3];
+  total = total_of[0] + total_of[1] + total_of[2] + total_of[3];
+  const bool on = counts(b);
+  if (threadIdx.x == 0) {
+    if (b == 0) *s.count = total;
+    if (b >= total) s.row_of[b] = -1;
+    if (on) s.row_of[before] = b;
+    if (b < s.R) {
+      s.compact_of[b] = on ? before : -1;
+      if (!on) s.loss[b] = 0.0f;
+      if (!s.divergence) {
+        const long long v = load_id(t.ids, t.ids_i64, b);
+        s.list_id[b] = on ? static_cast<int>(v) : INT_MAX;
+        if (!on && v != t.ignore_index) record_error(s.status, kErrBadIndex);
+      }
+    }
+  }
+  const int vecs = s.H / 8;
+  if (b >= total) {
+    uint4* dst = reinterpret_cast<uint4*>(s.hc + static_cast<long long>(b) * s.H);
+    for (int i = threadIdx.x; i < vecs; i += 128) dst[i] = make_uint4(0, 0, 0, 0);
+  }
+  if (on) {
+    const uint4* src = reinterpret_cast<const uint4*>(s.h + static_cast<long long>(b) * s.ldh);
+    uint4* dst = reinterpret_cast<uint4*>(s.hc + static_cast<long long>(before) * s.H);
+    for (int i = threadIdx.x; i < vecs; i += 128) dst[i] = src[i];
+  }
+}
+
 __global__ void __launch_bounds__(128) gather_rows_kernel(const HeadLossState s) {
   pdl_trigger();
   pdl_wait();
@@ -997,44 +1080,65 @@ __device__ __forceinline__ double warp_sum_f64(double v) {
   return v;
 }
 
-// Folds the tiles of a row and forms its loss (one warp a row).  The normaliser and the loss
-// are formed in fp64 from fp32 sums: a divergence is a small difference of logarithms.
+// Block-wide combinations of one value a thread (128 threads); `buf` holds four values.
+template <typename T, typename Op>
+__device__ __forceinline__ T block_combine(T v, T* buf, Op op) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+  __syncthreads();
+  if (threadIdx.x % 32 == 0) buf[threadIdx.x / 32] = v;
+  __syncthreads();
+  return op(op(buf[0], buf[1]), op(buf[2], buf[3]));
+}
+
+// Folds the tiles of a row and forms its loss (one block a row).  The normaliser and the loss are formed
+// in fp64 from fp32 sums: a divergence is a small difference of logarithms.
+//
+// The tensor core's sums of H products come out a little short (its additions truncate: about 2e-6 of a
+// logit at H = 3584).  Listed logits and normaliser share that, so most of it cancels in a loss; listed
+// logits summed again in fp32 made the losses worse (1.2e-6 for 0.9e-6 relative, 64 rows of 152064).
 __global__ void __launch_bounds__(128) finish_rows_kernel(const HeadLossState s, const HeadStatsScratch p) {
+  __shared__ double buf_d[4];
+  __shared__ float buf_f[4];
   pdl_trigger();
   pdl_wait();
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int m = blockIdx.x * 4 + warp;
+  const int tid = threadIdx.x;
+  const int m = blockIdx.x;
   if (m >= *s.count) return;
+  const auto add = [](double u, double v) { return u + v; };
+  const auto larger = [](float u, float v) { return fmaxf(u, v); };
   const int r = s.row_of[m];
   const float itf = s.inv_temp != nullptr ? s.inv_temp[r] : 1.0f;
   const double it = itf;
   const float c2 = itf * kLog2e;
   const float2* part = p.part + static_cast<long long>(m) * p.tiles;
   float mx = -INFINITY;
-  for (int i = lane; i < p.tiles; i += 32) mx = fmaxf(mx, part[i].x);
-  mx = warp_max(mx);
-  double rest = 0.0, plain = 0.0;
-  for (int i = lane; i < p.tiles; i += 32) {
+#pragma unroll 4
+  for (int i = tid; i < p.tiles; i += 128) mx = fmaxf(mx, part[i].x);
+  mx = block_combine(mx, buf_f, larger);
+  double part_rest = 0.0, plain = 0.0;
+#pragma unroll 4
+  for (int i = tid; i < p.tiles; i += 128) {
     const float2 v = part[i];
-    if (v.x != -INFINITY || !(v.y == 0.0f)) rest += static_cast<double>(v.y) * exp2f((v.x - mx) * c2);
+    if (v.x != -INFINITY || !(v.y == 0.0f)) part_rest += static_cast<double>(v.y) * exp2f((v.x - mx) * c2);
     if (p.part_sum != nullptr) plain += p.part_sum[static_cast<long long>(m) * p.tiles + i];
   }
-  rest = warp_sum_f64(rest);
-  if (p.part_sum != nullptr) plain = warp_sum_f64(plain);
+  part_rest = block_combine(part_rest, buf_d, add);
+  if (p.part_sum != nullptr) plain = block_combine(plain, buf_d, add);
   const long long base = static_cast<long long>(r) * s.K;
   float top = mx;
-  for (int k = lane; k < s.K; k += 32)
+  for (int k = tid; k < s.K; k += 128)
     if (s.list_id[base + k] != INT_MAX) top = fmaxf(top, s.list_logit[base + k]);
-  top = warp_max(top);
+  top = block_combine(top, buf_f, larger);
   double listed = 0.0;
-  for (int k = lane; k < s.K; k += 32)
+  for (int k = tid; k < s.K; k += 128)
     if (s.list_id[base + k] != INT_MAX)
       listed += exp((static_cast<double>(s.list_logit[base + k]) - static_cast<double>(top)) * it);
-  listed = warp_sum_f64(listed);
-  if (mx != -INFINITY) rest *= exp((static_cast<double>(mx) - static_cast<double>(top)) * it);
-  const double total = rest + listed;
-  const double lse = static_cast<double>(top) * it + log(total);
-  const double q_rest = rest / total;
+  listed = block_combine(listed, buf_d, add);
+  const double rest =
+      mx != -INFINITY ? part_rest * exp((static_cast<double>(mx) - static_cast<double>(top)) * it) : part_rest;
+  const double lse = static_cast<double>(top) * it + log(rest + listed);
+  const double q_rest = rest / (rest + listed);
   double loss, factor;
   if (!s.divergence) {
     const double target = s.list_logit[base];
@@ -1045,13 +1149,13 @@ __global__ void __launch_bounds__(128) finish_rows_kernel(const HeadLossState s,
     factor = 1.0 + 2.0 * s.z_loss * lse;
   } else {
     double sum = 0.0;
-    for (int k = lane; k < s.K; k += 32) {
+    for (int k = tid; k < s.K; k += 128) {
       if (s.list_id[base + k] == INT_MAX) continue;
       const double mass = s.list_mass[base + k];
       if (mass == 0.0) continue;
       sum += mass * (log(mass) - (static_cast<double>(s.list_logit[base + k]) * it - lse));
     }
-    loss = warp_sum_f64(sum);
+    loss = block_combine(sum, buf_d, add);
     factor = 1.0;
     const double rest_mass = s.rest_bucket ? static_cast<double>(s.rest_mass[r]) : 0.0;
     // a list of all columns leaves no rest; a teacher mass there is rounding
@@ -1060,7 +1164,7 @@ __global__ void __launch_bounds__(128) finish_rows_kernel(const HeadLossState s,
       factor = 1.0 - rest_mass / q_rest;
     }
   }
-  if (lane == 0) {
+  if (tid == 0) {
     s.loss[r] = static_cast<float>(loss);
     s.row_stat[r] = make_float4(static_cast<float>(lse), static_cast<float>(q_rest), static_cast<float>(factor), 0.0f);
   }
@@ -1079,23 +1183,10 @@ __global__ void __launch_bounds__(128) grad_rows_kernel(const HeadLossState s, c
     return;
   }
   const int r = s.row_of[m];
-  const float4 st = s.row_stat[r];
-  const float it = s.inv_temp != nullptr ? s.inv_temp[r] : 1.0f;
-  const float up = g.g[r] * it;
-  const float flat = s.divergence ? 0.0f : s.smoothing / static_cast<float>(s.V);
-  if (lane == 0) g.row_coef[m] = make_float4(it * kLog2e, st.x * kLog2e, up * st.z, up * flat);
+  if (lane == 0) g.row_coef[m] = row_coefficients(s, g.g, r);
   const long long base = static_cast<long long>(r) * s.K;
-  for (int k = lane; k < s.K; k += 32) {
-    if (s.list_id[base + k] == INT_MAX) continue;
-    float v;
-    if (s.divergence) {
-      v = expf(s.list_logit[base + k] * it - st.x) - s.list_mass[base + k];
-    } else {
-      // a p - 1 with p - 1 = -(mass of the rest): no cancellation in sure rows
-      v = (st.z - 1.0f) * (1.0f - st.y) - st.y + s.smoothing - flat;
-    }
-    g.list_grad[base + k] = up * v;
-  }
+  for (int k = lane; k < s.K; k += 32)
+    if (s.list_id[base + k] != INT_MAX) g.list_grad[base + k] = listed_gradient(s, g.g, r, base + k);
 }
 
 __global__ void __launch_bounds__(128) hidden_grad_kernel(const HeadLossState s, const HeadGradArgs g) {
@@ -1258,6 +1349,7 @@ cudaError_t head_loss_rows_launch(const HeadLossState& s, const HeadTargets& t, 
     e = launch_pdl(teacher_rows_kernel, dim3(ceil_div(s.R, 4)), dim3(128), smem, stream, s, t);
     if (e != cudaSuccess) return e;
   }
+  if (few_rows(s.R)) return launch_pdl(few_rows_kernel, dim3(s.rpad), dim3(128), 0, stream, s, t);
   e = launch_pdl(compact_rows_kernel, dim3(1), dim3(1024), 0, stream, s, t);
   if (e != cudaSuccess) return e;
   return launch_pdl(gather_rows_kernel, dim3(s.rpad), dim3(128), 0, stream, s);
@@ -1288,18 +1380,21 @@ cudaError_t head_loss_forward_launch(const HeadLossState& s, const HeadStatsScra
     e = launch_gemm<kStats, false>(maps, a, ceil_div(s.R, kBM) * a.tiles_n, stream);
   }
   if (e != cudaSuccess) return e;
-  return launch_pdl(finish_rows_kernel, dim3(ceil_div(s.R, 4)), dim3(128), 0, stream, s, p);
+  return launch_pdl(finish_rows_kernel, dim3(s.R), dim3(128), 0, stream, s, p);
 }
 
 cudaError_t head_loss_backward_launch(const HeadLossState& s, const HeadGradArgs& g, cudaStream_t stream) {
-  cudaError_t e = launch_pdl(grad_rows_kernel, dim3(ceil_div(s.rpad, 4)), dim3(128), 0, stream, s, g);
+  const bool dh = g.dh != nullptr, dw = g.dw != nullptr, few = few_rows(s.R);
+  cudaError_t e = cudaSuccess;
+  if (!few) e = launch_pdl(grad_rows_kernel, dim3(ceil_div(s.rpad, 4)), dim3(128), 0, stream, s, g);
   if (e != cudaSuccess) return e;
   Maps gm{}, pm{};
-  const bool dh = g.dh != nullptr, dw = g.dw != nullptr, few = few_rows(s.R);
   GemmArgs base = base_args(s);
   base.piece = g.piece;
   base.list_grad = g.list_grad;
   base.row_coef = g.row_coef;
+  base.s = s;
+  base.g = g.g;
   base.do_dh = dh;
   base.do_dw = dw;
   base.splits = g.splits;

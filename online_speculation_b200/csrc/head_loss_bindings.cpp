@@ -103,6 +103,7 @@ std::tuple<Tensor, Tensor> head_loss_forward(Tensor h, Tensor weight, Tensor ids
   TORCH_CHECK(ids.dim() == (divergence ? 2 : 1) && ids.size(0) == R, "one row of ids for every row of h");
   const int64_t K = divergence ? ids.size(1) : 1;
   c10::cuda::CUDAGuard guard(h.device());
+  check(cudaSetDevice(h.get_device()), "cudaSetDevice");   // see head_loss_backward
   const Tensor rows = tile_rows(h), w = tile_rows(weight);
   osb::HeadLossState s = make_state(w, R, H, K, inv_temp, divergence, given(teacher_lse), smoothing, z_loss, status);
   const auto bytes = h.options().dtype(torch::kUInt8), floats = h.options().dtype(torch::kFloat32);
@@ -159,6 +160,9 @@ std::tuple<OptTensor, OptTensor> head_loss_backward(Tensor saved, Tensor weight,
   TORCH_CHECK(g.is_cuda() && g.scalar_type() == torch::kFloat32 && g.is_contiguous() && g.dim() == 1, "g: one float per row");
   const int64_t R = g.size(0), H = weight.size(1), V = weight.size(0);
   c10::cuda::CUDAGuard guard(weight.device());
+  // binds the device's context to this thread: the tensor maps are made by the driver, which needs one, and
+  // an autograd thread may not have called the runtime yet
+  check(cudaSetDevice(weight.get_device()), "cudaSetDevice");
   const Tensor w = tile_rows(weight);
   osb::HeadLossState s = make_state(w, R, H, K, inv_temp, divergence, rest_bucket, smoothing, z_loss, status);
   TORCH_CHECK(saved.scalar_type() == torch::kUInt8 && saved.numel() == static_cast<int64_t>(bind_state(s, nullptr)),
@@ -198,6 +202,48 @@ std::tuple<OptTensor, OptTensor> head_loss_backward(Tensor saved, Tensor weight,
   a.list_grad = c.take<float>(R * K);
   check(osb::head_loss_backward_launch(s, a, at::cuda::getCurrentCUDAStream()), "head loss backward");
   return {dh, dw};
+}
+
+// The loss as an autograd node: the backward pass runs on the engine's thread without the interpreter.
+struct HeadLossNode : public torch::autograd::Function<HeadLossNode> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& h, const Tensor& weight, const Tensor& ids,
+                        const OptTensor& teacher, const OptTensor& teacher_lse, const OptTensor& inv_temp,
+                        int64_t ignore_index, double smoothing, double z_loss, int64_t piece, const Tensor& status) {
+    auto [loss, saved] = head_loss_forward(h, weight, ids, teacher, teacher_lse, inv_temp, ignore_index, smoothing,
+                                           z_loss, status);
+    ctx->save_for_backward({saved, weight, given(inv_temp) ? *inv_temp : Tensor(), status});
+    ctx->saved_data["k"] = given(teacher) ? ids.size(1) : 1;
+    ctx->saved_data["divergence"] = given(teacher);
+    ctx->saved_data["rest"] = given(teacher_lse);
+    ctx->saved_data["smoothing"] = smoothing;
+    ctx->saved_data["z"] = z_loss;
+    ctx->saved_data["piece"] = piece;
+    return loss;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "the head losses are differentiable once: create_graph is not supported");
+    const auto saved = ctx->get_saved_variables();
+    const Tensor g = grads[0].to(torch::kFloat32).contiguous();
+    OptTensor inv_temp;
+    if (saved[2].defined()) inv_temp = saved[2];
+    auto& d = ctx->saved_data;
+    auto [dh, dw] = head_loss_backward(saved[0], saved[1], inv_temp, g, d["k"].toInt(), d["divergence"].toBool(),
+                                       d["rest"].toBool(), d["smoothing"].toDouble(), d["z"].toDouble(),
+                                       ctx->needs_input_grad(0), ctx->needs_input_grad(1), d["piece"].toInt(), saved[3]);
+    torch::autograd::variable_list out(11);
+    if (given(dh)) out[0] = *dh;
+    if (given(dw)) out[1] = *dw;
+    return out;
+  }
+};
+
+Tensor head_loss(const Tensor& h, const Tensor& weight, const Tensor& ids, const OptTensor& teacher,
+                 const OptTensor& teacher_lse, const OptTensor& inv_temp, int64_t ignore_index, double smoothing,
+                 double z_loss, int64_t piece, const Tensor& status) {
+  return HeadLossNode::apply(h, weight, ids, teacher, teacher_lse, inv_temp, ignore_index, smoothing, z_loss, piece,
+                             status);
 }
 
 std::tuple<Tensor, Tensor, Tensor> top_logits(Tensor logits, int64_t k, OptTensor inv_temp) {
@@ -244,7 +290,6 @@ std::tuple<Tensor, Tensor, Tensor> top_logits(Tensor logits, int64_t k, OptTenso
 }  // namespace
 
 void register_head_losses(pybind11::module_& m) {
-  m.def("head_loss_forward", &head_loss_forward);
-  m.def("head_loss_backward", &head_loss_backward);
+  m.def("head_loss", &head_loss);
   m.def("top_logits", &top_logits);
 }

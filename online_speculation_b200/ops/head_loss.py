@@ -17,7 +17,6 @@ from __future__ import annotations
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _ext, workspace
 
@@ -55,27 +54,11 @@ def _check_rows(name, t, shape, dtypes, device):
 _INDEX = (torch.int32, torch.int64)
 
 
-class _HeadLoss(torch.autograd.Function):
-    """Forward: row lists, compaction, the statistics GEMM, the row losses.  Backward: per
-    vocabulary piece the gradient of its logits and the two products with it."""
-
-    @staticmethod
-    def forward(ctx, h, weight, ids, teacher, teacher_lse, inv_temp, ignore_index, smoothing, z_loss, piece):
-        status = workspace.status(h.device)
-        loss, saved = _ext.require().head_loss_forward(h, weight, ids, teacher, teacher_lse, inv_temp, ignore_index,
-                                                       smoothing, z_loss, status)
-        if ctx.needs_input_grad[0] or ctx.needs_input_grad[1]:
-            ctx.save_for_backward(saved, weight, inv_temp)
-            ctx.rest = (1 if teacher is None else ids.shape[1], teacher is not None, teacher_lse is not None, smoothing,
-                        z_loss, ctx.needs_input_grad[0], ctx.needs_input_grad[1], piece or 0, status)
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        saved, weight, inv_temp = ctx.saved_tensors
-        dh, dw = _ext.require().head_loss_backward(saved, weight, inv_temp, g.float().contiguous(), *ctx.rest)
-        return (dh, dw) + (None,) * 8
+def _head_loss(h, weight, ids, teacher, teacher_lse, inv_temp, ignore_index, smoothing, z_loss, piece):
+    """The extension's autograd node.  Forward: row lists, compaction, the statistics GEMM, the row losses.
+    Backward: per vocabulary piece the gradient of its logits and the two products with it."""
+    return _ext.require().head_loss(h, weight, ids, teacher, teacher_lse, inv_temp, ignore_index, smoothing, z_loss,
+                                    piece or 0, workspace.status(h.device))
 
 
 def head_cross_entropy(h: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *, ignore_index: int = -100,
@@ -102,8 +85,8 @@ def head_cross_entropy(h: torch.Tensor, weight: torch.Tensor, targets: torch.Ten
     if h.shape[0] == 0:
         return _empty_loss(h, weight)
     if h.is_cuda:
-        return _HeadLoss.apply(h, weight, targets.contiguous(), None, None, None, int(ignore_index),
-                               float(label_smoothing), float(z_loss), piece)
+        return _head_loss(h, weight, targets.contiguous(), None, None, None, int(ignore_index),
+                          float(label_smoothing), float(z_loss), piece)
     return _cross_entropy_reference(h, weight, targets, ignore_index, label_smoothing, z_loss)
 
 
@@ -138,9 +121,9 @@ def head_topk_divergence(h: torch.Tensor, weight: torch.Tensor, ids: torch.Tenso
         return _empty_loss(h, weight)
     teacher = teacher.detach()
     if h.is_cuda:
-        return _HeadLoss.apply(h, weight, ids.contiguous(), teacher.contiguous(),
-                               None if teacher_lse is None else teacher_lse.detach().contiguous(),
-                               None if inv_temp is None else inv_temp.detach().contiguous(), 0, 0.0, 0.0, piece)
+        return _head_loss(h, weight, ids.contiguous(), teacher.contiguous(),
+                          None if teacher_lse is None else teacher_lse.detach().contiguous(),
+                          None if inv_temp is None else inv_temp.detach().contiguous(), 0, 0.0, 0.0, piece)
     return _topk_divergence_reference(h, weight, ids, teacher, inv_temp, teacher_lse)
 
 
