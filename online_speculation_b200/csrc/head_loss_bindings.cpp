@@ -3,6 +3,8 @@
 // Scratch and saved tensors come from PyTorch's allocator on every call: two graphs, or two
 // streams, never share them.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -18,6 +20,18 @@ using OptTensor = c10::optional<Tensor>;
 void check(cudaError_t e, const char* what) {
   TORCH_CHECK(e == cudaSuccess, what, " failed: ", cudaGetErrorString(e));
 }
+
+// A tensor on the current device, past the dispatcher: small calls are bound by the host.
+Tensor device_tensor(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
+}
+
+// Bytes of the current stream that live as long as the call.
+struct Scratch {
+  c10::DataPtr data;
+  explicit Scratch(size_t bytes) : data(c10::cuda::CUDACachingAllocator::get()->allocate(bytes)) {}
+  char* base() const { return static_cast<char*>(data.get()); }
+};
 
 bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
 
@@ -106,12 +120,11 @@ std::tuple<Tensor, Tensor> head_loss_forward(Tensor h, Tensor weight, Tensor ids
   check(cudaSetDevice(h.get_device()), "cudaSetDevice");   // see head_loss_backward
   const Tensor rows = tile_rows(h), w = tile_rows(weight);
   osb::HeadLossState s = make_state(w, R, H, K, inv_temp, divergence, given(teacher_lse), smoothing, z_loss, status);
-  const auto bytes = h.options().dtype(torch::kUInt8), floats = h.options().dtype(torch::kFloat32);
-  Tensor saved = torch::empty({static_cast<int64_t>(bind_state(s, nullptr))}, bytes);
+  Tensor saved = device_tensor({static_cast<int64_t>(bind_state(s, nullptr))}, torch::kUInt8, h);
   bind_state(s, static_cast<char*>(saved.data_ptr()));
   s.h = reinterpret_cast<const __nv_bfloat16*>(rows.data_ptr());
   s.ldh = row_stride(rows);
-  Tensor loss = torch::empty({R}, floats);
+  Tensor loss = device_tensor({R}, torch::kFloat32, h);
   s.loss = loss.data_ptr<float>();
 
   osb::HeadTargets t{};
@@ -139,8 +152,8 @@ std::tuple<Tensor, Tensor> head_loss_forward(Tensor h, Tensor weight, Tensor ids
   size.take<float2>(parts);
   size.take<float>(smoothing != 0.0 ? parts : 0);
   size.take<unsigned char>(R);
-  Tensor scratch = torch::empty({static_cast<int64_t>(size.at)}, bytes);
-  Carve c{static_cast<char*>(scratch.data_ptr())};
+  const Scratch scratch(size.at);
+  Carve c{scratch.base()};
   p.part = c.take<float2>(parts);
   float* part_sum = c.take<float>(smoothing != 0.0 ? parts : 0);
   p.part_sum = smoothing != 0.0 ? part_sum : nullptr;
@@ -177,14 +190,13 @@ std::tuple<OptTensor, OptTensor> head_loss_backward(Tensor saved, Tensor weight,
     a.piece = osb::head_loss_piece(s.R, s.V);
   }
   a.splits = need_dh ? osb::head_loss_splits(s.R, s.H, a.piece, s.V, need_dw) : 1;
-  const auto opts = weight.options();
   OptTensor dh, dw;
   if (need_dh) {
-    dh = torch::empty({R, H}, opts);
+    dh = device_tensor({R, H}, torch::kBFloat16, weight);
     a.dh = reinterpret_cast<__nv_bfloat16*>(dh->data_ptr());
   }
   if (need_dw) {
-    dw = torch::empty({V, H}, opts);
+    dw = device_tensor({V, H}, torch::kBFloat16, weight);
     a.dw = reinterpret_cast<__nv_bfloat16*>(dw->data_ptr());
   }
   const long long dl = static_cast<long long>(osb::head_loss_grad_rows(s.R)) * a.piece;
@@ -194,8 +206,8 @@ std::tuple<OptTensor, OptTensor> head_loss_backward(Tensor saved, Tensor weight,
   size.take<float>(parts);
   size.take<float4>(s.rpad);
   size.take<float>(R * K);
-  Tensor scratch = torch::empty({static_cast<int64_t>(size.at)}, opts.dtype(torch::kUInt8));
-  Carve c{static_cast<char*>(scratch.data_ptr())};
+  const Scratch scratch(size.at);
+  Carve c{scratch.base()};
   a.dl = c.take<__nv_bfloat16>(dl);
   a.dh_part = c.take<float>(parts);
   a.row_coef = c.take<float4>(s.rpad);
@@ -259,9 +271,8 @@ std::tuple<Tensor, Tensor, Tensor> top_logits(Tensor logits, int64_t k, OptTenso
     a.inv_temp = inv_temp->data_ptr<float>();
   }
   c10::cuda::CUDAGuard guard(logits.device());
-  const auto floats = logits.options().dtype(torch::kFloat32);
-  Tensor values = torch::empty({R, k}, floats), ids = torch::empty({R, k}, floats.dtype(torch::kInt32));
-  Tensor lse = torch::empty({R}, floats);
+  Tensor values = device_tensor({R, k}, torch::kFloat32, logits), ids = device_tensor({R, k}, torch::kInt32, logits);
+  Tensor lse = device_tensor({R}, torch::kFloat32, logits);
   a.logits = logits.data_ptr();
   a.bf16 = logits.scalar_type() == torch::kBFloat16;
   a.ld = row_stride(logits);
@@ -273,13 +284,13 @@ std::tuple<Tensor, Tensor, Tensor> top_logits(Tensor logits, int64_t k, OptTenso
   a.values = values.data_ptr<float>();
   a.ids = ids.data_ptr<int>();
   a.lse = lse.data_ptr<float>();
-  Tensor scratch;
+  c10::optional<Scratch> scratch;
   if (a.splits > 1) {
     Carve size{nullptr};
     size.take<unsigned long long>(R * a.splits * k);
     size.take<float2>(R * a.splits);
-    scratch = torch::empty({static_cast<int64_t>(size.at)}, floats.dtype(torch::kUInt8));
-    Carve c{static_cast<char*>(scratch.data_ptr())};
+    scratch.emplace(size.at);
+    Carve c{scratch->base()};
     a.keys = c.take<unsigned long long>(R * a.splits * k);
     a.part = c.take<float2>(R * a.splits);
   }
