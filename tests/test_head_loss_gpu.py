@@ -145,7 +145,8 @@ def _teacher(rows, vocab, k, gen, cuda, dtype, ragged):
 
 
 @pytest.mark.parametrize("rows,hidden,vocab,k", [(1, 8, 1, 1), (1, 64, 500, 1), (3, 72, 40, 40), (50, 512, 2048, 8),
-                                                 (130, 136, 777, 64), (40, 64, 3001, 512), (260, 200, 1030, 17)])
+                                                 (130, 136, 777, 64), (40, 64, 3001, 512), (260, 200, 1030, 17),
+                                                 (256, 64, 600, 512), (100, 72, 9000, 100), (257, 64, 512, 512)])
 @pytest.mark.parametrize("rest,temp,ragged,dtype,piece", [(False, False, False, torch.float32, None),
                                                           (True, True, True, torch.float32, 256),
                                                           (True, False, False, torch.bfloat16, 512),
@@ -291,6 +292,74 @@ def test_teacher_to_student(cuda):
     for got, i in ((h.grad, 2), (w.grad, 4)):
         want = a[i] + b[i]
         oracle.within(got, want, a[i + 1] + b[i + 1] + oracle.BF16_HALF * (want.abs() + a[i].abs() + b[i].abs()), i)
+
+
+def test_many_rows_and_pieces(cuda):
+    """More rows than one block numbers at a time, an odd number of them counting, several pieces."""
+    rows, hidden, vocab = 2500, 64, 1800
+    h, w, t, gen = oracle.make_inputs(rows, hidden, vocab, 13, cuda)
+    t[torch.rand(rows, generator=gen).to(cuda) < 0.45] = -100
+    g = torch.randn(rows, generator=gen).to(cuda)
+    want = oracle.cross_entropy(h, w, t, g)
+    h.requires_grad_()
+    w.requires_grad_()
+    for piece in (None, 768):
+        loss = K.head_cross_entropy(h, w, t, piece=piece)
+        dh, dw = _grads(loss, h, w, g)
+        for got, i, name in ((loss.detach(), 0, "loss"), (dh, 2, "dh"), (dw, 4, "dW")):
+            oracle.within(got, want[i], want[i + 1], name)
+
+
+def test_two_streams_at_once(cuda):
+    """Eager calls in flight on two streams share no scratch."""
+    cases = []
+    for i, rows in enumerate((220, 700)):
+        h, w, t, gen = oracle.make_inputs(rows, 128, 5000, 50 + i, cuda)
+        g = torch.randn(rows, generator=gen).to(cuda)
+        want = oracle.cross_entropy(h, w, t, g)
+        logits = torch.randn(rows, 30000, generator=gen).to(cuda)
+        cases.append((h.requires_grad_(), w.requires_grad_(), t, g, want, logits, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    results = [[], []]
+    for _ in range(4):
+        for i, (h, w, t, g, _, logits, stream) in enumerate(cases):
+            with torch.cuda.stream(stream):
+                loss = K.head_cross_entropy(h, w, t, piece=512)
+                results[i].append((loss.detach(), *_grads(loss, h, w, g), K.top_logits(logits, 20)))
+    torch.cuda.synchronize()
+    for (h, w, t, g, want, logits, _), runs in zip(cases, results):
+        values, ids, _ = _top_reference(logits, 20)
+        for loss, dh, dw, top in runs:
+            for got, j in ((loss, 0), (dh, 2), (dw, 4)):
+                oracle.within(got, want[j], want[j + 1], j)
+            assert torch.equal(top[1].cpu().long(), ids) and torch.equal(top[0].cpu(), values)
+
+
+def test_gradient_rules(cuda):
+    """Once differentiable; a head changed between the passes is noticed; the graph can be kept."""
+    h, w, t, gen = oracle.make_inputs(20, 64, 300, 14, cuda)
+    h.requires_grad_()
+    w.requires_grad_()
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(K.head_cross_entropy(h, w, t).sum(), [h], create_graph=True)
+    loss = K.head_cross_entropy(h, w, t)
+    a = torch.autograd.grad(loss.sum(), [h, w], retain_graph=True)
+    b = torch.autograd.grad(loss.sum(), [h, w], retain_graph=True)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    with torch.no_grad():
+        w.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(loss.sum(), [h])
+    assert not K.head_cross_entropy(h.detach(), w.detach(), t).requires_grad
+
+
+def test_empty_batch(cuda):
+    h = torch.zeros(0, 64, dtype=torch.bfloat16, device=cuda, requires_grad=True)
+    w = torch.zeros(9, 64, dtype=torch.bfloat16, device=cuda, requires_grad=True)
+    loss = K.head_cross_entropy(h, w, torch.zeros(0, dtype=torch.long, device=cuda))
+    dh, dw = torch.autograd.grad(loss, [h, w], torch.zeros(0, device=cuda))
+    assert loss.shape == (0,) and dh.shape == (0, 64) and bool((dw == 0).all())
+    assert K.top_logits(torch.zeros(0, 9, device=cuda), 3)[0].shape == (0, 3)
 
 
 def test_repeats_are_bitwise_equal(cuda):
