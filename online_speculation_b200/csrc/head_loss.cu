@@ -25,6 +25,10 @@
 //   lanes and rows in its columns.  A pass over few rows is the reading of the head, and a tile of
 //   256 lanes that holds 64 rows would spend four times the matrix instructions (and the clock that
 //   their power costs: 93 % tensor-pipe active at 1.5 GHz for 64 rows) on lanes that nobody looks at.
+// * Up to 128 rows keep dl as the sum of two bf16 numbers.  A row's gradient is mostly its target's
+//   entry: with few rows the rounding of single entries shows in the results (0.0027 relative where the
+//   rounding of the outputs alone is 0.0017), and the second half is nearly free, as the head is read
+//   all the same.  With many rows the errors average out and the products would double.
 #include "common.cuh"
 #include "head_loss.h"
 
@@ -45,6 +49,7 @@ constexpr int kOutBytes = 32 * 128;       // one warp's staged output box: 32 ro
 constexpr int kThreads = 192;             // TMA warp, MMA warp, four epilogue warps
 constexpr int kOutTotal = 4 * 2 * kOutBytes;
 constexpr int kFewRows = 256;             // rows that fit the accumulator's columns
+constexpr int kSplitRows = 128;           // rows whose logits' gradient is kept in two bf16 halves
 // Per-row state of the passes with rows in columns, behind the output boxes: running maximum and sum and
 // plain sum (one set a warp), list cursors (one set a warp), coefficients, row numbers.
 constexpr int kStateMax = 0, kStateSum = kStateMax + 4 * kFewRows * 4, kStatePlain = kStateSum + 4 * kFewRows * 4,
@@ -68,6 +73,8 @@ struct GemmArgs {
   int v0, cols;            // this piece: first vocabulary row, columns that exist
   int bn;                  // rows in columns: how many columns, a multiple of 16
   int tiles_n;             // column tiles of the accumulator grid
+  int lo;                  // rows in columns: where a row of the logits' gradient holds what rounding to bf16 took
+                           // from its first half (0: not kept)
   int slot;                // rows in columns: vocabulary columns in the lanes of one CTA (statistics: a multiple of
                            // 8, gradient: of 32)
   int stages;              // of the ring
@@ -88,6 +95,10 @@ struct GemmArgs {
   int* status;
 };
 
+// Rows in columns, hidden gradient: boxes of 64 rows that one CTA stages, its half of the rows or, in two
+// halves, all rows of one of them.
+__host__ __device__ inline int row_boxes(const GemmArgs& a) { return ((a.lo > 0 ? a.bn : a.bn / 2) + 63) / 64; }
+
 struct StageBytes {
   int a, b;
 };
@@ -95,12 +106,13 @@ struct StageBytes {
 // Shared memory of one stage: this CTA's part of either operand.
 __host__ __device__ inline StageBytes stage_bytes_of(int mode, bool few, const GemmArgs& a) {
   if (few && mode != kProd) return {a.slot * kRowBytes, a.bn / 2 * kRowBytes};
-  if (few && !a.do_dw) return {kHalf * kRowBytes, (a.bn / 2 + 63) / 64 * kBox};
+  if (few && !a.do_dw) return {kHalf * kRowBytes, row_boxes(a) * kBox};
   return {kHalf * kRowBytes, kHalf * kRowBytes};
 }
 
 __host__ __device__ inline int out_bytes_of(int mode, bool few) {
-  return mode == kStats ? (few ? kOutTotal / 2 : 0) : kOutTotal;
+  if (mode == kProd || !few) return mode == kStats ? 0 : kOutTotal;
+  return mode == kStats ? kOutTotal / 2 : kOutTotal + kOutTotal / 2;   // a block for listed logits, next to the boxes
 }
 
 // One work item: an accumulator tile and its range of reduction blocks.
@@ -135,7 +147,7 @@ __device__ __forceinline__ bool item_at(const GemmArgs& a, int rows, int pair, i
   // The hidden gradient's items reduce over the piece, the head gradient's over the rows, and cost
   // accordingly: the former go first, dealt around; the pairs that got one less take as many of the
   // latter in its place as weigh the same, and the rest is dealt around.
-  const int kb = (a.cols + kBK - 1) / kBK, per = (kb + a.splits - 1) / a.splits, kbw = (rows + kBK - 1) / kBK;
+  const int kb = (a.cols + kBK - 1) / kBK, per = (kb + a.splits - 1) / a.splits, kbw = (rows + kBK - 1) / kBK * (FEW && a.lo > 0 ? 2 : 1);
   const int per_split = FEW ? (rows > 0 ? a.tiles_n : 0) : tm * a.tiles_n;   // a.tiles_n tiles across the hidden width
   const int nh = a.do_dh ? per_split * a.splits : 0;
   const int nw = a.do_dw ? ((a.cols + kBM - 1) / kBM) * a.tiles_n : 0;
@@ -392,7 +404,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           const uint32_t bar = map_shared_rank(smem_u32(&full[stage]), 0);
           const int k0 = kb * kBK;
           const bool hidden = MODE == kProd && it.kind == 0;
-          const int rows_box = (a.bn / 2 + 63) / 64;   // rows in columns: boxes of 64 rows
+          const int rows_box = row_boxes(a);
           if (rank == 0) {
             const int bytes = MODE != kProd ? stage_bytes
                               : FEW && hidden ? kHalf * kRowBytes + rows_box * kBox
@@ -407,8 +419,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             for (int j = 0; j < kHalf / 64; ++j)
               pair_load_2d(pa + j * kBox, &maps.a0, it.m0 + rank * kHalf + j * 64, a.v0 + k0, bar);
             for (int j = 0; j < rows_box; ++j)
-              pair_load_2d(pb + j * kBox, &maps.b0, rank * (a.bn / 2) + j * 64, k0, bar);
+              pair_load_2d(pb + j * kBox, &maps.b0, rank * (a.lo > 0 ? a.lo : a.bn / 2) + j * 64, k0, bar);
           } else {
+            // head gradient in two halves: the second half's blocks meet the same rows again
+            const int over = k0 - (FEW && a.lo > 0 ? (rows + kBK - 1) / kBK * kBK : INT_MAX);
+            const int ka = over >= 0 ? a.lo + over : k0, kh = over >= 0 ? over : k0;
             const int ma = it.m0 + rank * kHalf, nb = it.n0 + rank * kHalf;
             if (MODE != kProd) {
               pair_load_2d(pa, &maps.a0, k0, ma, bar);
@@ -418,11 +433,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int j = 0; j < kHalf / 64; ++j) pair_load_2d(pb + j * kBox, &maps.b0, nb + j * 64, a.v0 + k0, bar);
             } else {
-              if (FEW) pair_load_2d(pa, &maps.a1, k0, ma, bar);
+              if (FEW) pair_load_2d(pa, &maps.a1, ka, ma, bar);
 #pragma unroll
               for (int j = 0; j < kHalf / 64; ++j) {
                 if (!FEW) pair_load_2d(pa + j * kBox, &maps.a1, ma + j * 64, k0, bar);
-                pair_load_2d(pb + j * kBox, &maps.b1, nb + j * 64, k0, bar);
+                pair_load_2d(pb + j * kBox, &maps.b1, nb + j * 64, kh, bar);
               }
             }
           }
@@ -458,7 +473,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         tc_fence_after();
         const uint32_t d = tmem + acc * kBN;
         const bool mn_a = MODE == kProd && (it.kind == (FEW ? 0 : 1)), mn_b = MODE == kProd;
-        const int columns = FEW && it.kind == 0 ? a.bn : kBN;
+        const int columns = FEW && it.kind == 0 ? (MODE == kProd && a.lo > 0 ? 2 * a.bn : a.bn) : kBN;
         const uint32_t idesc = idesc_bf16_f32(kBM, columns) | (mn_a ? 1u << 15 : 0u) | (mn_b ? 1u << 16 : 0u);
         for (int kb = it.kb0; kb < it.kb1; ++kb) {
           if (!mbar_wait(&full[stage], phase, a.status, kErrMmaWait)) {
@@ -615,9 +630,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             sums[t] = sums[t] * kept + s;
             __syncwarp();
           } else {
-            uint8_t* box = out + (staged & 1) * kOutBytes;
+            // one box at a time in turn, or both for the two halves
+            uint8_t* box = out + (a.lo > 0 ? 0 : (staged & 1) * kOutBytes);
             if ((c & 1) == 0) {
-              if (lane == 0) bulk_wait_read<1>();
+              if (lane == 0) {
+                if (a.lo > 0) bulk_wait_read<0>();
+                else bulk_wait_read<1>();
+              }
               __syncwarp();
             }
 #pragma unroll
@@ -625,14 +644,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
               const float4 k = coef_of[t0 + j];
               x[j] = k.z * ex2(fmaf(x[j], k.x, -k.y)) - k.w;
             }
-            // the other box, once its store has read it, holds the block
-            int2 peek = t < rows ? cursors[t] : make_int2(0, INT_MAX);
-            if (__any_sync(0xffffffffu, peek.y < min(first + 32, stop))) {
-              if (lane == 0) bulk_wait_read<0>();
-              __syncwarp();
-              listed(x, t, out + ((staged + 1) & 1) * kOutBytes,
-                     [&](float* at, long long k) { *at = listed_gradient(a.s, a.g, row_no[t], k); });
-            }
+            listed(x, t, sOut + kOutTotal + quarter * kOutBytes,
+                   [&](float* at, long long k) { *at = listed_gradient(a.s, a.g, row_no[t], k); });
             if (t0 + 32 > rows) {
               // columns behind the rows hold what an earlier tile left
 #pragma unroll
@@ -644,12 +657,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
               const uint4 v = make_uint4(pack2(x[8 * q], x[8 * q + 1]), pack2(x[8 * q + 2], x[8 * q + 3]),
                                          pack2(x[8 * q + 4], x[8 * q + 5]), pack2(x[8 * q + 6], x[8 * q + 7]));
               *reinterpret_cast<uint4*>(box + swizzled(lane, (c & 1) * 4 + q)) = on ? v : make_uint4(0, 0, 0, 0);
+              if (a.lo > 0) {
+                const unsigned hi[4] = {v.x, v.y, v.z, v.w};
+                unsigned low[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  low[e] = pack2(x[8 * q + 2 * e] - __uint_as_float(hi[e] << 16),
+                                 x[8 * q + 2 * e + 1] - __uint_as_float(hi[e] & 0xFFFF0000u));
+                *reinterpret_cast<uint4*>(box + kOutBytes + swizzled(lane, (c & 1) * 4 + q)) =
+                    on ? make_uint4(low[0], low[1], low[2], low[3]) : make_uint4(0, 0, 0, 0);
+              }
             }
             if (c & 1) {
               fence_proxy_async_smem();
               __syncwarp();
               if (lane == 0) {
                 tma_store_2d(&maps.out0, box, (c >> 1) * 64, m0);
+                if (a.lo > 0) tma_store_2d(&maps.out0, box + kOutBytes, a.lo + (c >> 1) * 64, m0);
                 bulk_commit();
               }
               ++staged;
@@ -660,7 +684,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           // behind the vocabulary, but inside a block that the hidden gradient's product reads: zeros
           for (int c = 0; c < (rows + 63) / 64; ++c) {
             uint8_t* box = out + (staged & 1) * kOutBytes;
-            if (lane == 0) bulk_wait_read<1>();
+            if (lane == 0) bulk_wait_read<0>();
             __syncwarp();
 #pragma unroll
             for (int q = 0; q < 8; ++q) *reinterpret_cast<uint4*>(box + swizzled(lane, q)) = make_uint4(0, 0, 0, 0);
@@ -668,6 +692,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             __syncwarp();
             if (lane == 0) {
               tma_store_2d(&maps.out0, box, c * 64, m0);
+              if (a.lo > 0) tma_store_2d(&maps.out0, box, a.lo + c * 64, m0);
               bulk_commit();
             }
             ++staged;
@@ -767,6 +792,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         for (int c = 0; c < (rows + 31) / 32 && m0 < a.H; ++c) {
           float x[32];
           tmem_ld32(t_acc + c * 32, x);
+          if (a.lo > 0) {
+            float y[32];
+            tmem_ld32(t_acc + a.bn + c * 32, y);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) x[j] += y[j];
+          }
           uint8_t* box = out + (staged & 1) * kOutBytes;
           if (lane == 0) bulk_wait_read<1>();
           __syncwarp();
@@ -1074,12 +1105,6 @@ __global__ void __launch_bounds__(128) gather_rows_kernel(const HeadLossState s)
   for (int i = threadIdx.x; i < vecs; i += 128) dst[i] = src[i];
 }
 
-__device__ __forceinline__ double warp_sum_f64(double v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
 // Block-wide combinations of one value a thread (128 threads); `buf` holds four values.
 template <typename T, typename Op>
 __device__ __forceinline__ T block_combine(T v, T* buf, Op op) {
@@ -1297,6 +1322,7 @@ GemmArgs base_args(const HeadLossState& s) {
   a.rpad = s.rpad;
   a.slot = kHalf;
   a.bn = few_rows(s.R) ? ceil_div(s.R, 16) * 16 : kBN;
+  a.lo = s.R <= kSplitRows ? ceil_div(s.R, 64) * 64 : 0;
   a.status = s.status;
   return a;
 }
@@ -1308,8 +1334,12 @@ int head_loss_vocab_tiles(int R, int V) {
   return few_rows(R) ? 8 * pairs_for(ceil_div(V, 2 * lane_slot(V, 8))) : ceil_div(V, kBN);
 }
 
-// Row pitch or row count of the logits' gradient: [piece][few rows] or [rows][piece].
-int head_loss_grad_rows(int R) { return few_rows(R) ? ceil_div(R, 64) * 64 : ceil_div(R, kHeadRowPad) * kHeadRowPad; }
+// Row pitch or row count of the logits' gradient: [piece][few rows, in two halves up to kSplitRows] or
+// [rows][piece].
+int head_loss_grad_rows(int R) {
+  if (R <= kSplitRows) return 2 * ceil_div(R, 64) * 64;
+  return few_rows(R) ? ceil_div(R, 64) * 64 : ceil_div(R, kHeadRowPad) * kHeadRowPad;
+}
 
 // Columns of the logits that the backward pass works on at a time.  Their gradient takes two bytes a row and
 // column: 256 MB of it, so that a pass over a piece is long against the ends of its two launches.
@@ -1325,7 +1355,8 @@ int head_loss_piece(int R, int V) {
 int head_loss_splits(int R, int H, int piece, int V, bool with_dw) {
   const int pairs = device_sms() / 2, cols = std::min(piece, V), kb = ceil_div(cols, kBK);
   const long long tiles = static_cast<long long>(few_rows(R) ? 1 : ceil_div(R, kBM)) * ceil_div(H, kBN);
-  const long long other = static_cast<long long>(ceil_div(cols, kBM)) * ceil_div(H, kBN) * ceil_div(R, kBK);
+  const long long other =
+      static_cast<long long>(ceil_div(cols, kBM)) * ceil_div(H, kBN) * ceil_div(R, kBK) * (R <= kSplitRows ? 2 : 1);
   int best = 1;
   long long cost = LLONG_MAX;
   for (int want = 1; want <= 16 && want * 4 <= std::max(kb, 4); ++want) {
