@@ -46,8 +46,11 @@ constexpr int kMaxStages = 12;
 constexpr int kRowBytes = kBK * 2;        // one staged row of either operand
 constexpr int kBox = 64 * 64 * 2;         // one MN-major box: 64 reduction rows of 64 elements
 constexpr int kOutBytes = 32 * 128;       // one warp's staged output box: 32 rows of 128 bytes
-constexpr int kThreads = 192;             // TMA warp, MMA warp, four epilogue warps
-constexpr int kOutTotal = 4 * 2 * kOutBytes;
+// Epilogue warps: four cover the accumulator's lanes.  With rows in lanes there are two sets, each for half of
+// the columns: below about 600 hidden columns a tile's products take less time than one set needs for it.
+constexpr int epilogue_warps(bool few) { return few ? 4 : 8; }
+constexpr int threads_of(bool few) { return 64 + 32 * epilogue_warps(few); }   // TMA warp, MMA warp, epilogue
+constexpr int kOutTotal = 8 * kOutBytes;  // two boxes a warp, or one with twice the warps
 constexpr int kFewRows = 256;             // rows that fit the accumulator's columns
 constexpr int kSplitRows = 128;           // rows whose logits' gradient is kept in two bf16 halves
 // Per-row state of the passes with rows in columns, behind the output boxes: running maximum and sum and
@@ -335,7 +338,7 @@ __device__ __forceinline__ float* block_at(uint8_t* buf, int row, int col) {
 }
 
 template <int MODE, bool FEW>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(FEW), 1)
     head_gemm_kernel(const __grid_constant__ Maps maps, const GemmArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -364,7 +367,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tfull[i], 1);
-      mbar_init(&tempty[i], 8);   // the epilogue warps of both CTAs
+      mbar_init(&tempty[i], 2 * epilogue_warps(FEW));   // of both CTAs
     }
     mbar_init(drain, 1);
     fence_barrier_init();
@@ -507,7 +510,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------ epilogue
     const int quarter = warp % 4;
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
-    uint8_t* out = sOut + quarter * 2 * kOutBytes;
+    const int set = (warp - 2) / 4;                         // its half of the columns (rows in lanes)
+    constexpr int kBoxes = FEW ? 2 : 1;                     // output boxes of a warp
+    uint8_t* out = sOut + (FEW ? quarter * 2 : warp - 2) * kOutBytes;
+    auto next_box = [&](int staged) {
+      // the box's last store has read it
+      if (lane == 0) bulk_wait_read<kBoxes - 1>();
+      __syncwarp();
+      return out + (staged & (kBoxes - 1)) * kOutBytes;
+    };
     int acc = 0, staged = 0;
     uint32_t acc_phase = 0;
     if (FEW && MODE != kProd) {
@@ -561,7 +572,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           list0 = static_cast<long long>(o) * a.K;
           if (MODE == kStats && a.inv_temp != nullptr) c2 = a.inv_temp[o] * kLog2e;
           if (MODE == kGrad) coef = a.row_coef[m];
-          cur.seek(a.list_id + list0, a.K, a.v0 + it.n0);
+          cur.seek(a.list_id + list0, a.K, a.v0 + it.n0 + set * (kBN / 2));
         }
       }
       if (!empty_sum) {
@@ -701,7 +712,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       } else if (MODE == kStats) {
         float mx = -INFINITY, sum = 0.0f, plain = 0.0f;
         const int end = min(a.V, it.n0 + kBN);         // behind the tile's last column
-        for (int c = 0; c < kBN / 32; ++c) {
+        for (int c = set * (kBN / 64); c < (set + 1) * (kBN / 64); ++c) {
           const int col = it.n0 + c * 32;              // vocabulary column of x[0]
           if (col >= end || m0 >= rows) break;
           float x[32];
@@ -741,16 +752,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           mx = top;
         }
         if (live) {
-          const long long p = static_cast<long long>(m) * a.part_tiles + it.n0 / kBN;
+          const long long p = static_cast<long long>(m) * a.part_tiles + 2 * (it.n0 / kBN) + set;
           a.part[p] = make_float2(mx, sum);
           if (a.part_sum != nullptr) a.part_sum[p] = plain;
         }
       } else if (MODE == kGrad) {
         // the whole tile is written: the products read its rows up to the tile's end
-        for (int c = 0; c < kBN / 64; ++c) {
-          uint8_t* box = out + (staged & 1) * kOutBytes;
-          if (lane == 0) bulk_wait_read<1>();
-          __syncwarp();
+        for (int c = set * (kBN / 128); c < (set + 1) * (kBN / 128); ++c) {
+          uint8_t* box = next_box(staged);
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             float x[32];
@@ -798,9 +807,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int j = 0; j < 32; ++j) x[j] += y[j];
           }
-          uint8_t* box = out + (staged & 1) * kOutBytes;
-          if (lane == 0) bulk_wait_read<1>();
-          __syncwarp();
+          uint8_t* box = next_box(staged);
 #pragma unroll
           for (int j = 0; j < 32; ++j) *block_at(box, j, lane) = x[j];
           fence_proxy_async_smem();
@@ -817,13 +824,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
       } else if (it.kind == 0) {
         // hidden gradient: fp32, added to what earlier pieces left
-        for (int c = 0; c < kBN / 32; ++c) {
+        for (int c = set * (kBN / 64); c < (set + 1) * (kBN / 64); ++c) {
+          if (it.n0 + c * 32 >= a.H) break;
           float x[32];
           tmem_ld32(t_acc + c * 32, x);
-          if (it.n0 + c * 32 >= a.H) break;
-          uint8_t* box = out + (staged & 1) * kOutBytes;
-          if (lane == 0) bulk_wait_read<1>();
-          __syncwarp();
+          uint8_t* box = next_box(staged);
 #pragma unroll
           for (int q = 0; q < 8; ++q)
             *reinterpret_cast<float4*>(box + swizzled(lane, q)) =
@@ -843,11 +848,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       } else {
         // head gradient of the piece: complete, rounded once
         const bool in_rows = a.v0 + m0 < a.V;
-        for (int c = 0; c < kBN / 64; ++c) {
+        constexpr int kSpan = kBN / 64 / (epilogue_warps(FEW) / 4);
+        for (int c = set * kSpan; c < (set + 1) * kSpan; ++c) {
           if (it.n0 + c * 64 >= a.H) break;
-          uint8_t* box = out + (staged & 1) * kOutBytes;
-          if (lane == 0) bulk_wait_read<1>();
-          __syncwarp();
+          uint8_t* box = next_box(staged);
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             float x[32];
@@ -1308,7 +1312,7 @@ cudaError_t launch_gemm(const Maps& maps, GemmArgs a, int max_items, cudaStream_
   const StageBytes sb = stage_bytes_of(MODE, FEW, a);
   a.stages = std::min(kMaxStages, (kSmemMost - rest) / (sb.a + sb.b));
   const int smem = 1024 + a.stages * (sb.a + sb.b) + rest;
-  return launch_pdl(head_gemm_kernel<MODE, FEW>, dim3(2 * pairs_for(max_items)), dim3(kThreads), smem, stream, maps, a);
+  return launch_pdl(head_gemm_kernel<MODE, FEW>, dim3(2 * pairs_for(max_items)), dim3(threads_of(FEW)), smem, stream, maps, a);
 }
 
 GemmArgs base_args(const HeadLossState& s) {
@@ -1329,9 +1333,9 @@ GemmArgs base_args(const HeadLossState& s) {
 
 }  // namespace
 
-// Partial statistics per row: one a warp of the launch, or one a tile of columns.
+// Partial statistics per row: one a warp of the launch, or two a tile of columns.
 int head_loss_vocab_tiles(int R, int V) {
-  return few_rows(R) ? 8 * pairs_for(ceil_div(V, 2 * lane_slot(V, 8))) : ceil_div(V, kBN);
+  return few_rows(R) ? 8 * pairs_for(ceil_div(V, 2 * lane_slot(V, 8))) : 2 * ceil_div(V, kBN);
 }
 
 // Row pitch or row count of the logits' gradient: [piece][few rows, in two halves up to kSplitRows] or
