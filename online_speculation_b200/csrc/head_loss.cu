@@ -220,6 +220,34 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Two fp32 operations an instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+      "add.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+      "mul.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmov.b64 rc, {%6, %7};\n\t"
+      "fma.rn.f32x2 rd, ra, rb, rc;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int x, int y) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
                    reinterpret_cast<uint64_t>(map)),
@@ -542,8 +570,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(FEW), 1)
     const int* row_no = reinterpret_cast<const int*>(state + kStateRow);
     const float4* coef_of = reinterpret_cast<const float4*>(state + kStateCoef);
     int2* cursors = reinterpret_cast<int2*>(state + kStateCursor) + quarter * kFewRows;
-    Item it;
-    for (int i = 0; item_at<MODE, FEW>(a, rows, pair, pairs, i, it); ++i) {
+    // Row inputs of the next tile are fetched while this one is worked on: its row, its first listed column (all
+    // that a list of one has), its coefficients.
+    int next_row = -1, next_id = INT_MAX;
+    float4 next_coef = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    auto fetch_row = [&](const Item& n) {
+      const int m = n.m0 + rank * kHalf + quarter * 32 + lane;
+      next_row = m < rows ? a.row_of[m] : -1;
+      if (MODE == kGrad && m < rows) next_coef = a.row_coef[m];
+    };
+    float next_scale = kLog2e;
+    auto fetch_id = [&]() {
+      next_id = next_row >= 0 ? a.list_id[static_cast<long long>(next_row) * a.K] : INT_MAX;
+      if (MODE == kStats && next_row >= 0 && a.inv_temp != nullptr) next_scale = a.inv_temp[next_row] * kLog2e;
+    };
+    Item it, ahead;
+    bool more = item_at<MODE, FEW>(a, rows, pair, pairs, 0, ahead);
+    if (!FEW && MODE != kProd && more) {
+      fetch_row(ahead);
+      fetch_id();
+    }
+    for (int i = 0; more; ++i) {
+      it = ahead;
+      more = item_at<MODE, FEW>(a, rows, pair, pairs, i + 1, ahead);
       const int held = FEW && MODE != kProd ? a.slot : kHalf;
       const int m0 = it.m0 + rank * held + quarter * 32;    // first tile row of this warp
       const int m = m0 + lane;
@@ -564,16 +613,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(FEW), 1)
         __syncwarp();
       } else if (MODE != kProd) {
         live = m < rows;
+        coef = next_coef;
+        const int o = next_row, col = a.v0 + it.n0 + set * (kBN / 2);
+        list0 = static_cast<long long>(o) * a.K;
+        cur.ids = a.list_id + list0;
+        cur.K = live ? a.K : 0;
         cur.k = 0;
-        cur.K = 0;
-        cur.next = INT_MAX;
-        if (live) {
-          const int o = a.row_of[m];
-          list0 = static_cast<long long>(o) * a.K;
-          if (MODE == kStats && a.inv_temp != nullptr) c2 = a.inv_temp[o] * kLog2e;
-          if (MODE == kGrad) coef = a.row_coef[m];
-          cur.seek(a.list_id + list0, a.K, a.v0 + it.n0 + set * (kBN / 2));
+        cur.next = next_id;
+        if (live && next_id < col) {
+          if (a.K == 1) cur.next = INT_MAX;
+          else cur.seek(cur.ids, a.K, col);
         }
+        c2 = next_scale;
+        if (more) fetch_row(ahead);
       }
       if (!empty_sum) {
         const bool ok = __all_sync(0xffffffffu, mbar_wait(&tfull[acc], acc_phase, a.status, kErrEpilogueWait));
@@ -740,15 +792,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(FEW), 1)
             cur.advance();
           }
           __syncwarp();
-          float top = mx;
+          float tops[4] = {mx, x[1], x[2], x[3]};
 #pragma unroll
-          for (int j = 0; j < 32; ++j) top = fmaxf(top, x[j]);
+          for (int j = 0; j < 32; ++j) tops[j & 3] = fmaxf(tops[j & 3], x[j]);
+          const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
           const float ref = top == -INFINITY ? 0.0f : top;
           sum *= ex2((mx - ref) * c2);
-          float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          const float2 minus = make_float2(-ref, -ref), scale = make_float2(c2, c2);
+          float2 s2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-          for (int j = 0; j < 32; ++j) s4[j & 3] += ex2((x[j] - ref) * c2);
-          sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+          for (int j = 0; j < 16; ++j) {
+            const float2 d = mul2(add2(make_float2(x[2 * j], x[2 * j + 1]), minus), scale);
+            s2[j & 1] = add2(s2[j & 1], make_float2(ex2(d.x), ex2(d.y)));
+          }
+          sum += (s2[0].x + s2[1].x) + (s2[0].y + s2[1].y);
           mx = top;
         }
         if (live) {
@@ -766,7 +823,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(FEW), 1)
             tmem_ld32(t_acc + c * 64 + half * 32, x);
             const int col = a.v0 + it.n0 + c * 64 + half * 32;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) x[j] = coef.z * ex2(fmaf(x[j], coef.x, -coef.y)) - coef.w;
+            for (int j = 0; j < 16; ++j) {
+              float2 d = fma2(make_float2(x[2 * j], x[2 * j + 1]), make_float2(coef.x, coef.x), make_float2(-coef.y, -coef.y));
+              d = fma2(make_float2(ex2(d.x), ex2(d.y)), make_float2(coef.z, coef.z), make_float2(-coef.w, -coef.w));
+              x[2 * j] = d.x;
+              x[2 * j + 1] = d.y;
+            }
             while (cur.next < col + 32) {
               const int at = cur.next - col;
               const float v = a.list_grad[list0 + cur.k];
@@ -878,6 +940,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(FEW), 1)
           ++staged;
         }
       }
+      if (!FEW && MODE != kProd && more) fetch_id();
       if (!empty_sum) {
         tc_fence_before();
         __syncwarp();
