@@ -54,10 +54,11 @@ constexpr int kOutTotal = 8 * kOutBytes;  // two boxes a warp, or one with twice
 constexpr int kFewRows = 256;             // rows that fit the accumulator's columns
 constexpr int kSplitRows = 128;           // rows whose logits' gradient is kept in two bf16 halves
 // Per-row state of the passes with rows in columns, behind the output boxes: running maximum and sum and
-// plain sum (one set a warp), list cursors (one set a warp), coefficients, row numbers.
+// plain sum (one set a warp), list cursors (one set a warp), coefficients, row numbers, factor or value of listed gradients.
 constexpr int kStateMax = 0, kStateSum = kStateMax + 4 * kFewRows * 4, kStatePlain = kStateSum + 4 * kFewRows * 4,
               kStateCursor = kStatePlain + 4 * kFewRows * 4, kStateCoef = kStateCursor + 4 * kFewRows * 8,
-              kStateRow = kStateCoef + kFewRows * 16, kStateBytes = kStateRow + kFewRows * 4;
+              kStateRow = kStateCoef + kFewRows * 16, kStateListed = kStateRow + kFewRows * 4,
+              kStateBytes = kStateListed + kFewRows * 4;
 constexpr int kBarBytes = 256;            // barriers and the TMEM address
 constexpr int kSmemMost = 232448 - 1024;               // behind the alignment
 constexpr float kLog2e = 1.4426950408889634f;
@@ -166,7 +167,10 @@ __device__ __forceinline__ bool item_at(const GemmArgs& a, int rows, int pair, i
   }
   int j = i - mine, t;
   const int late = extra > 0 ? pairs - extra : 0;   // pairs with one less
-  const int each = late > 0 && kbw > 0 ? min((per + kbw / 2) / kbw, nw / late) : 0;
+  // in blocks: a head gradient's tile takes as long as eight at least, for its end and its output; a hidden
+  // gradient's block over few rows waits for the head, half again as long as its products
+  const int weigh = max(kbw, 8), weigh_hidden = FEW ? per + per / 2 : per;
+  const int each = late > 0 && kbw > 0 ? min((weigh_hidden + weigh / 2) / weigh, nw / late) : 0;
   if (late > 0 && pair >= extra && j < each) {
     t = pair - extra + j * late;
   } else {
@@ -277,24 +281,34 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 // Position of 16-byte chunk c of row r in a 128-byte-swizzled box of 32 rows.
 __device__ __forceinline__ int swizzled(int r, int c) { return r * 128 + (((c ^ r) & 7) << 4); }
 
-// A row's cursor into its ascending list of columns.
+// A row's cursor into its ascending list of columns.  The column behind the next one, and the next one's
+// value, are on their way before they are needed.
 struct ListCursor {
   const int* ids;
-  int k, K, next;
-  __device__ __forceinline__ void seek(const int* p, int count, int col) {
-    ids = p;
-    K = count;
-    int lo = 0, hi = count;
+  const float* values;       // or null
+  int k, K, next, after;
+  float value;
+  __device__ __forceinline__ int id(int i) const { return i < K ? ids[i] : INT_MAX; }
+  __device__ __forceinline__ void load() {
+    next = id(k);
+    after = id(k + 1);
+    value = values != nullptr && k < K ? values[k] : 0.0f;
+  }
+  // The first column at or behind `col`, not before the `from`-th.
+  __device__ __forceinline__ void seek(int from, int col) {
+    int lo = from, hi = K;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
       if (ids[mid] < col) lo = mid + 1; else hi = mid;
     }
     k = lo;
-    next = k < K ? ids[k] : INT_MAX;
+    load();
   }
   __device__ __forceinline__ void advance() {
     ++k;
-    next = k < K ? ids[k] : INT_MAX;
+    next = after;
+    after = id(k + 1);
+    value = values != nullptr && k < K ? values[k] : 0.0f;
   }
 };
 
@@ -554,7 +568,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(FEW), 1)
         const int o = t < rows ? a.row_of[t] : -1;
         reinterpret_cast<int*>(state + kStateRow)[t] = o;
         float4 c = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (MODE == kGrad && o >= 0) c = row_coefficients(a.s, a.g, o);
+        if (MODE == kGrad && o >= 0) {
+          c = row_coefficients(a.s, a.g, o);
+          reinterpret_cast<float*>(state + kStateListed)[t] =
+              a.s.divergence ? a.g[o] * (a.s.inv_temp != nullptr ? a.s.inv_temp[o] : 1.0f)
+                             : listed_gradient(a.s, a.g, o, o);
+        }
         if (MODE == kStats) c.x = (o >= 0 && a.inv_temp != nullptr ? a.inv_temp[o] : 1.0f) * kLog2e;
         reinterpret_cast<float4*>(state + kStateCoef)[t] = c;
       }
@@ -569,6 +588,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(FEW), 1)
     }
     const int* row_no = reinterpret_cast<const int*>(state + kStateRow);
     const float4* coef_of = reinterpret_cast<const float4*>(state + kStateCoef);
+    const float* listed_of = reinterpret_cast<const float*>(state + kStateListed);
     int2* cursors = reinterpret_cast<int2*>(state + kStateCursor) + quarter * kFewRows;
     // Row inputs of the next tile are fetched while this one is worked on: its row, its first listed column (all
     // that a list of one has), its coefficients.
@@ -607,7 +627,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(FEW), 1)
       if (FEW && MODE != kProd) {
         // every row's place in its list, for this warp's vocabulary columns
         for (int t = lane; t < rows; t += 32) {
-          cur.seek(a.list_id + static_cast<long long>(row_no[t]) * a.K, a.K, a.v0 + m0);
+          cur.ids = a.list_id + static_cast<long long>(row_no[t]) * a.K;
+          cur.values = nullptr;
+          cur.K = a.K;
+          cur.seek(0, a.v0 + m0);
           cursors[t] = make_int2(cur.k, cur.next);
         }
         __syncwarp();
@@ -617,12 +640,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(FEW), 1)
         const int o = next_row, col = a.v0 + it.n0 + set * (kBN / 2);
         list0 = static_cast<long long>(o) * a.K;
         cur.ids = a.list_id + list0;
+        cur.values = MODE == kGrad ? a.list_grad + list0 : nullptr;
         cur.K = live ? a.K : 0;
         cur.k = 0;
         cur.next = next_id;
-        if (live && next_id < col) {
-          if (a.K == 1) cur.next = INT_MAX;
-          else cur.seek(cur.ids, a.K, col);
+        if (next_id >= col) {
+          cur.after = cur.id(1);
+          cur.value = MODE == kGrad && live ? cur.values[0] : 0.0f;
+        } else if (a.K == 1) {
+          cur.next = INT_MAX;
+        } else {
+          cur.seek(1, col);
         }
         c2 = next_scale;
         if (more) fetch_row(ahead);
@@ -649,10 +677,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(FEW), 1)
           if (!__any_sync(0xffffffffu, c.y < end)) return;
           spill_block(buf, x);
           const long long base = t < rows ? static_cast<long long>(row_no[t]) * a.K : 0;
+          int after = c.y < end && c.x + 1 < a.K ? a.list_id[base + c.x + 1] : INT_MAX;
           while (c.y < end) {
-            use(block_at(buf, c.y - first, lane), base + c.x);
+            const int here = c.y - first, k = c.x;
             ++c.x;
-            c.y = c.x < a.K ? a.list_id[base + c.x] : INT_MAX;
+            c.y = after;
+            after = c.x + 1 < a.K ? a.list_id[base + c.x + 1] : INT_MAX;
+            use(block_at(buf, here, lane), base + k);
           }
           reload_block(buf, x);
         };
@@ -708,7 +739,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(FEW), 1)
               x[j] = k.z * ex2(fmaf(x[j], k.x, -k.y)) - k.w;
             }
             listed(x, t, sOut + kOutTotal + quarter * kOutBytes,
-                   [&](float* at, long long k) { *at = listed_gradient(a.s, a.g, row_no[t], k); });
+                   [&](float* at, long long k) {
+                     const float4 f = coef_of[t];
+                     *at = a.s.divergence
+                               ? listed_of[t] * (ex2(fmaf(a.s.list_logit[k], f.x, -f.y)) - a.s.list_mass[k])
+                               : listed_of[t];
+                   });
             if (t0 + 32 > rows) {
               // columns behind the rows hold what an earlier tile left
 #pragma unroll
@@ -831,7 +867,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(FEW), 1)
             }
             while (cur.next < col + 32) {
               const int at = cur.next - col;
-              const float v = a.list_grad[list0 + cur.k];
+              const float v = cur.value;
 #pragma unroll
               for (int j = 0; j < 32; ++j)
                 if (j == at) x[j] = v;
@@ -974,24 +1010,39 @@ __device__ __forceinline__ long long load_id(const void* p, int i64, long long i
   return i64 ? static_cast<const long long*>(p)[i] : static_cast<const int*>(p)[i];
 }
 
-// The teacher's list of one row (one warp): empty slots dropped, a column listed twice
-// merged, ascending by column; its masses in fp64, rounded to fp32.
+// Block-wide combinations of one value a thread (128 threads); `buf` holds four values.
+template <typename T, typename Op>
+__device__ __forceinline__ T block_combine(T v, T* buf, Op op) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+  __syncthreads();
+  if (threadIdx.x % 32 == 0) buf[threadIdx.x / 32] = v;
+  __syncthreads();
+  return op(op(buf[0], buf[1]), op(buf[2], buf[3]));
+}
+
+// The teacher's list of one row (one block): empty slots dropped, a column listed twice merged, ascending by
+// column (a bitonic sort; comparing all with all took 135 us for 3957 rows of 241); its masses in fp64,
+// rounded to fp32.
 __global__ void __launch_bounds__(128) teacher_rows_kernel(const HeadLossState s, const HeadTargets t) {
-  extern __shared__ uint8_t raw[];
+  __shared__ unsigned long long key[kHeadMaxListed];   // column above slot; empty slots above all
+  __shared__ double mass[kHeadMaxListed];
+  __shared__ double buf[4];
+  __shared__ int found[4];
   pdl_trigger();
   pdl_wait();
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int K = s.K;
-  double* mass = reinterpret_cast<double*>(raw) + static_cast<long long>(warp) * K;
-  int* id = reinterpret_cast<int*>(raw + static_cast<long long>(4) * K * 8) + warp * K;
-  int* key = id + 4 * K;
-  const int r = blockIdx.x * 4 + warp;
-  if (r >= s.R) return;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, K = s.K, r = blockIdx.x;
+  int size = 32;
+  while (size < K) size *= 2;
   const long long base = static_cast<long long>(r) * K;
   const double it = s.inv_temp != nullptr ? static_cast<double>(s.inv_temp[r]) : 1.0;
+  const auto add = [](double u, double v) { return u + v; };
+  const auto larger = [](double u, double v) { return fmax(u, v); };
   double top = -INFINITY;
   bool any = false, nan = false;
-  for (int k = lane; k < K; k += 32) {
+  for (int k = tid; k < size; k += 128) {
+    key[k] = ~0ull;
+    if (k >= K) continue;
     long long v = load_id(t.ids, t.ids_i64, base + k);
     const float x = t.teacher_bf16 ? bf2f(static_cast<const __nv_bfloat16*>(t.teacher)[base + k])
                                    : static_cast<const float*>(t.teacher)[base + k];
@@ -999,59 +1050,65 @@ __global__ void __launch_bounds__(128) teacher_rows_kernel(const HeadLossState s
       record_error(s.status, kErrBadIndex);
       v = -1;
     }
-    const bool has = v >= 0 && !(x == -INFINITY);
-    id[k] = has ? static_cast<int>(v) : INT_MAX;
-    const double z = has ? static_cast<double>(x) * it : -INFINITY;
+    mass[k] = -INFINITY;
+    if (v < 0 || x == -INFINITY) continue;
+    key[k] = (static_cast<unsigned long long>(v) << 32) | static_cast<unsigned>(k);
+    const double z = static_cast<double>(x) * it;
     mass[k] = z;
-    any |= has;
-    nan |= has && !(z == z);
+    any = true;
+    nan |= !(z == z);
     top = fmax(top, z);
   }
-  any = __any_sync(0xffffffffu, any);
-  nan = __any_sync(0xffffffffu, nan);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
+  any = __syncthreads_or(any);
+  nan = __syncthreads_or(nan);
+  top = block_combine(top, buf, larger);
   const double shift = t.teacher_lse != nullptr ? static_cast<double>(t.teacher_lse[r]) : top;
-  __syncwarp();
   double sum = 0.0;
-  for (int k = lane; k < K; k += 32) {
-    const double e = id[k] == INT_MAX ? 0.0 : exp(mass[k] - shift);
+  for (int k = tid; k < K; k += 128) {
+    const double e = key[k] == ~0ull ? 0.0 : exp(mass[k] - shift);
     mass[k] = e;
     sum += e;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  sum = block_combine(sum, buf, add);
   const double inv = t.teacher_lse != nullptr ? 1.0 : 1.0 / sum;
-  __syncwarp();
-  // first slot of every column takes the masses of its later ones
-  for (int k = lane; k < K; k += 32) {
-    const int v = id[k];
-    bool first = v != INT_MAX;
-#pragma unroll 8
-    for (int j = 0; j < K; ++j) first = first && !(id[j] == v && j < k);
-    key[k] = first ? v : INT_MAX;
-  }
-  __syncwarp();
-  for (int k = lane; k < K; k += 32) s.list_id[base + k] = INT_MAX;
-  __syncwarp();
-  for (int k = lane; k < K; k += 32) {
-    const int v = key[k];
-    if (v == INT_MAX) continue;
-    int at = 0;
-    int twins = 0;
-#pragma unroll 8
-    for (int j = 0; j < K; ++j) {
-      at += key[j] < v;
-      twins += id[j] == v;
+  for (int span = 2; span <= size; span *= 2) {
+    for (int step = span / 2; step > 0; step /= 2) {
+      __syncthreads();
+      for (int i = tid; i < size / 2; i += 128) {
+        const int at = 2 * i - (i & (step - 1)), other = at + step;
+        const unsigned long long u = key[at], v = key[other];
+        if ((u > v) == ((at & span) == 0)) {
+          key[at] = v;
+          key[other] = u;
+        }
+      }
     }
-    double m = mass[k];
-    if (twins > 1)
-      for (int j = k + 1; j < K; ++j)
-        if (id[j] == v) m += mass[j];
-    s.list_id[base + at] = v;
-    s.list_mass[base + at] = static_cast<float>(m * inv);
   }
-  if (lane == 0) {
+  __syncthreads();
+  int before = 0;
+  for (int i0 = 0; i0 < size; i0 += 128) {
+    const int i = i0 + tid;
+    const unsigned long long mine = i < size ? key[i] : ~0ull;
+    const unsigned column = static_cast<unsigned>(mine >> 32);
+    // the first of a column takes the masses of its later ones
+    const bool first = mine != ~0ull && (i == 0 || static_cast<unsigned>(key[i - 1] >> 32) != column);
+    const unsigned ballot = __ballot_sync(0xffffffffu, first);
+    __syncthreads();
+    if (lane == 0) found[warp] = __popc(ballot);
+    __syncthreads();
+    int at = before + __popc(ballot & ((1u << lane) - 1u));
+    for (int q = 0; q < warp; ++q) at += found[q];
+    if (first) {
+      double m = mass[static_cast<unsigned>(mine)];
+      for (int j = i + 1; j < size && static_cast<unsigned>(key[j] >> 32) == column; ++j)
+        m += mass[static_cast<unsigned>(key[j])];
+      s.list_id[base + at] = static_cast<int>(column);
+      s.list_mass[base + at] = static_cast<float>(m * inv);
+    }
+    before += found[0] + found[1] + found[2] + found[3];
+  }
+  for (int k = before + tid; k < K; k += 128) s.list_id[base + k] = INT_MAX;
+  if (tid == 0) {
     t.active[r] = any ? 1 : 0;
     const double rest = t.teacher_lse != nullptr ? (nan ? sum : fmax(1.0 - sum, 0.0)) : 0.0;
     s.rest_mass[r] = static_cast<float>(rest);
@@ -1170,17 +1227,6 @@ __global__ void __launch_bounds__(128) gather_rows_kernel(const HeadLossState s)
   }
   const uint4* src = reinterpret_cast<const uint4*>(s.h + static_cast<long long>(s.row_of[m]) * s.ldh);
   for (int i = threadIdx.x; i < vecs; i += 128) dst[i] = src[i];
-}
-
-// Block-wide combinations of one value a thread (128 threads); `buf` holds four values.
-template <typename T, typename Op>
-__device__ __forceinline__ T block_combine(T v, T* buf, Op op) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if (threadIdx.x % 32 == 0) buf[threadIdx.x / 32] = v;
-  __syncthreads();
-  return op(op(buf[0], buf[1]), op(buf[2], buf[3]));
 }
 
 // Folds the tiles of a row and forms its loss (one block a row).  The normaliser and the loss are formed
@@ -1421,15 +1467,17 @@ int head_loss_piece(int R, int V) {
 // everything; alone, as many as give every pair the same work.
 int head_loss_splits(int R, int H, int piece, int V, bool with_dw) {
   const int pairs = device_sms() / 2, cols = std::min(piece, V), kb = ceil_div(cols, kBK);
-  const long long tiles = static_cast<long long>(few_rows(R) ? 1 : ceil_div(R, kBM)) * ceil_div(H, kBN);
-  const long long other =
-      static_cast<long long>(ceil_div(cols, kBM)) * ceil_div(H, kBN) * ceil_div(R, kBK) * (R <= kSplitRows ? 2 : 1);
+  const bool few = few_rows(R);
+  const long long tiles = static_cast<long long>(few ? 1 : ceil_div(R, kBM)) * ceil_div(H, kBN);
+  const long long kbw = std::max(ceil_div(R, kBK) * (R <= kSplitRows ? 2 : 1), 8);     // weights: see item_at
+  const long long other = static_cast<long long>(ceil_div(cols, kBM)) * ceil_div(H, kBN) * kbw;
+  const long long bytes = 4ll * ceil_div(R, kHeadRowPad) * kHeadRowPad * H;             // of one partial sum
   int best = 1;
   long long cost = LLONG_MAX;
-  for (int want = 1; want <= 16 && want * 4 <= std::max(kb, 4); ++want) {
+  for (int want = 1; want <= pairs && want * 4 <= std::max(kb, 4) && (want == 1 || want * bytes <= (256ll << 20)); ++want) {
     if (want > 1 && tiles >= 2 * pairs) break;          // enough tiles as they are
-    const int per = ceil_div(kb, want), splits = ceil_div(kb, per);
-    if (with_dw && per <= (tiles * kb + other) / pairs) return splits;
+    const int per = ceil_div(kb, want), splits = ceil_div(kb, per), weigh = few ? per + per / 2 : per;
+    if (with_dw && weigh <= (tiles * weigh * splits + other) / pairs) return splits;
     // a tile's end and its partial sums weigh about four blocks
     const long long c = static_cast<long long>(ceil_div(tiles * splits, pairs)) * (per + 4);
     if (c < cost) {
@@ -1443,8 +1491,7 @@ int head_loss_splits(int R, int H, int piece, int V, bool with_dw) {
 cudaError_t head_loss_rows_launch(const HeadLossState& s, const HeadTargets& t, cudaStream_t stream) {
   cudaError_t e;
   if (s.divergence) {
-    const size_t smem = static_cast<size_t>(4) * s.K * (8 + 4 + 4);
-    e = launch_pdl(teacher_rows_kernel, dim3(ceil_div(s.R, 4)), dim3(128), smem, stream, s, t);
+    e = launch_pdl(teacher_rows_kernel, dim3(s.R), dim3(128), 0, stream, s, t);
     if (e != cudaSuccess) return e;
   }
   if (few_rows(s.R)) return launch_pdl(few_rows_kernel, dim3(s.rpad), dim3(128), 0, stream, s, t);

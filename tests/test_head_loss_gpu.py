@@ -146,7 +146,8 @@ def _teacher(rows, vocab, k, gen, cuda, dtype, ragged):
 
 @pytest.mark.parametrize("rows,hidden,vocab,k", [(1, 8, 1, 1), (1, 64, 500, 1), (3, 72, 40, 40), (50, 512, 2048, 8),
                                                  (130, 136, 777, 64), (40, 64, 3001, 512), (260, 200, 1030, 17),
-                                                 (256, 64, 600, 512), (100, 72, 9000, 100), (257, 64, 512, 512)])
+                                                 (256, 64, 600, 512), (100, 72, 9000, 100), (257, 64, 512, 512), (400, 64, 5000, 33),
+                                                 (20, 64, 140000, 200)])
 @pytest.mark.parametrize("rest,temp,ragged,dtype,piece", [(False, False, False, torch.float32, None),
                                                           (True, True, True, torch.float32, 256),
                                                           (True, False, False, torch.bfloat16, 512),
