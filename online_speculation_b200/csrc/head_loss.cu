@@ -46,10 +46,11 @@ constexpr int kMaxStages = 12;
 constexpr int kRowBytes = kBK * 2;        // one staged row of either operand
 constexpr int kBox = 64 * 64 * 2;         // one MN-major box: 64 reduction rows of 64 elements
 constexpr int kOutBytes = 32 * 128;       // one warp's staged output box: 32 rows of 128 bytes
-// Epilogue warps: four cover the accumulator's lanes.  With rows in lanes there are two sets, each for half of
-// the columns: below about 600 hidden columns a tile's products take less time than one set needs for it.
-constexpr int epilogue_warps(bool few) { return few ? 4 : 8; }
-constexpr int threads_of(bool few) { return 64 + 32 * epilogue_warps(few); }   // TMA warp, MMA warp, epilogue
+// Epilogue warps: four cover the accumulator's lanes.  Mostly there are two sets, each for half of the columns:
+// below about 600 hidden columns, or with few rows to reduce over, a tile's products take less time than
+// one set needs for it.  With rows in columns the logits' passes have one set, which holds the rows' state.
+constexpr int epilogue_warps(int mode, bool few) { return few && mode != 2 ? 4 : 8; }
+constexpr int threads_of(int mode, bool few) { return 64 + 32 * epilogue_warps(mode, few); }   // and TMA, MMA
 constexpr int kOutTotal = 8 * kOutBytes;  // two boxes a warp, or one with twice the warps
 constexpr int kFewRows = 256;             // rows that fit the accumulator's columns
 constexpr int kSplitRows = 128;           // rows whose logits' gradient is kept in two bf16 halves
@@ -115,7 +116,8 @@ __host__ __device__ inline StageBytes stage_bytes_of(int mode, bool few, const G
 }
 
 __host__ __device__ inline int out_bytes_of(int mode, bool few) {
-  if (mode == kProd || !few) return mode == kStats ? 0 : kOutTotal;
+  if (few && mode == kProd) return 2 * kOutTotal;
+  if (!few) return mode == kStats ? 0 : kOutTotal;
   return mode == kStats ? kOutTotal / 2 : kOutTotal + kOutTotal / 2;   // a block for listed logits, next to the boxes
 }
 
@@ -380,7 +382,7 @@ __device__ __forceinline__ float* block_at(uint8_t* buf, int row, int col) {
 }
 
 template <int MODE, bool FEW>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(FEW), 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW), 1)
     head_gemm_kernel(const __grid_constant__ Maps maps, const GemmArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -409,7 +411,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(FEW), 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tfull[i], 1);
-      mbar_init(&tempty[i], 2 * epilogue_warps(FEW));   // of both CTAs
+      mbar_init(&tempty[i], 2 * epilogue_warps(MODE, FEW));   // of both CTAs
     }
     mbar_init(drain, 1);
     fence_barrier_init();
@@ -552,9 +554,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(FEW), 1)
     // ------------------------------------------------------------ epilogue
     const int quarter = warp % 4;
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
-    const int set = (warp - 2) / 4;                         // its half of the columns (rows in lanes)
+    constexpr int kSets = epilogue_warps(MODE, FEW) / 4;
     constexpr int kBoxes = FEW ? 2 : 1;                     // output boxes of a warp
-    uint8_t* out = sOut + (FEW ? quarter * 2 : warp - 2) * kOutBytes;
+    const int set = (warp - 2) / 4;                         // its share of the columns
+    uint8_t* out = sOut + (kSets == 1 ? quarter : warp - 2) * kBoxes * kOutBytes;
     auto next_box = [&](int staged) {
       // the box's last store has read it
       if (lane == 0) bulk_wait_read<kBoxes - 1>();
@@ -896,7 +899,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(FEW), 1)
         }
       } else if (FEW && it.kind == 0) {
         // hidden gradient with hidden columns in the lanes: turned around on the way into the box
-        for (int c = 0; c < (rows + 31) / 32 && m0 < a.H; ++c) {
+        for (int c = set; c < (rows + 31) / 32 && m0 < a.H; c += kSets) {
           float x[32];
           tmem_ld32(t_acc + c * 32, x);
           if (a.lo > 0) {
@@ -946,7 +949,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(FEW), 1)
       } else {
         // head gradient of the piece: complete, rounded once
         const bool in_rows = a.v0 + m0 < a.V;
-        constexpr int kSpan = kBN / 64 / (epilogue_warps(FEW) / 4);
+        constexpr int kSpan = kBN / 64 / kSets;
         for (int c = set * kSpan; c < (set + 1) * kSpan; ++c) {
           if (it.n0 + c * 64 >= a.H) break;
           uint8_t* box = next_box(staged);
@@ -1421,7 +1424,7 @@ cudaError_t launch_gemm(const Maps& maps, GemmArgs a, int max_items, cudaStream_
   const StageBytes sb = stage_bytes_of(MODE, FEW, a);
   a.stages = std::min(kMaxStages, (kSmemMost - rest) / (sb.a + sb.b));
   const int smem = 1024 + a.stages * (sb.a + sb.b) + rest;
-  return launch_pdl(head_gemm_kernel<MODE, FEW>, dim3(2 * pairs_for(max_items)), dim3(threads_of(FEW)), smem, stream, maps, a);
+  return launch_pdl(head_gemm_kernel<MODE, FEW>, dim3(2 * pairs_for(max_items)), dim3(threads_of(MODE, FEW)), smem, stream, maps, a);
 }
 
 GemmArgs base_args(const HeadLossState& s) {
