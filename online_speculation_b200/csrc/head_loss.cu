@@ -1,4 +1,4 @@
-// Losses on a vocabulary head whose logits are never stored: softmax cross entropy and the
+// Losses on a vocabulary head whose logits are not stored (or, for few rows, once): softmax cross entropy and the
 // divergence from a teacher's listed logits, with the gradients of the hidden rows and of
 // the head.
 //
@@ -25,6 +25,8 @@
 //   lanes and rows in its columns.  A pass over few rows is the reading of the head, and a tile of
 //   256 lanes that holds 64 rows would spend four times the matrix instructions (and the clock that
 //   their power costs: 93 % tensor-pipe active at 1.5 GHz for 64 rows) on lanes that nobody looks at.
+//   Where those rows' logits are small next to the head, the forward pass leaves them for the backward pass,
+//   which then reads the head once instead of twice (head_loss_kept).
 // * Up to 128 rows keep dl as the sum of two bf16 numbers.  A row's gradient is mostly its target's
 //   entry: with few rows the rounding of single entries shows in the results (0.0027 relative where the
 //   rounding of the outputs alone is 0.0017), and the second half is nearly free, as the head is read
@@ -55,9 +57,9 @@ constexpr int kOutTotal = 8 * kOutBytes;  // two boxes a warp, or one with twice
 constexpr int kFewRows = 256;             // rows that fit the accumulator's columns
 constexpr int kSplitRows = 128;           // rows whose logits' gradient is kept in two bf16 halves
 // Per-row state of the passes with rows in columns, behind the output boxes: running maximum and sum and
-// plain sum (one set a warp), list cursors (one set a warp), coefficients, row numbers, factor or value of listed gradients.
+// plain sum (one set a warp), list cursors (one set a warp, two of the CTA), coefficients, row numbers, factor or value of listed gradients.
 constexpr int kStateMax = 0, kStateSum = kStateMax + 4 * kFewRows * 4, kStatePlain = kStateSum + 4 * kFewRows * 4,
-              kStateCursor = kStatePlain + 4 * kFewRows * 4, kStateCoef = kStateCursor + 4 * kFewRows * 8,
+              kStateCursor = kStatePlain + 4 * kFewRows * 4, kStateCoef = kStateCursor + 6 * kFewRows * 8,
               kStateRow = kStateCoef + kFewRows * 16, kStateListed = kStateRow + kFewRows * 4,
               kStateBytes = kStateListed + kFewRows * 4;
 constexpr int kBarBytes = 256;            // barriers and the TMEM address
@@ -92,6 +94,7 @@ struct GemmArgs {
   HeadLossState s;         // rows in columns, grad: coefficients and listed values are formed on the spot
   const float* g;
   const float* inv_temp;   // stats
+  int kept;                // stats with rows in columns: the logits are stored for the backward pass
   float2* part;
   float* part_sum;
   int part_tiles;
@@ -115,10 +118,10 @@ __host__ __device__ inline StageBytes stage_bytes_of(int mode, bool few, const G
   return {kHalf * kRowBytes, kHalf * kRowBytes};
 }
 
-__host__ __device__ inline int out_bytes_of(int mode, bool few) {
+__host__ __device__ inline int out_bytes_of(int mode, bool few, bool kept) {
   if (few && mode == kProd) return 2 * kOutTotal;
   if (!few) return mode == kStats ? 0 : kOutTotal;
-  return mode == kStats ? kOutTotal / 2 : kOutTotal + kOutTotal / 2;   // a block for listed logits, next to the boxes
+  return (mode == kStats && !kept ? 0 : kOutTotal) + kOutTotal / 2;   // a block for listed logits, behind the boxes
 }
 
 // One work item: an accumulator tile and its range of reduction blocks.
@@ -280,6 +283,16 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&p);
 }
 
+// What rounding eight values to bf16 took from them, rounded itself.
+__device__ __forceinline__ uint4 rounded_off(const float* x, uint4 hi) {
+  const unsigned h[4] = {hi.x, hi.y, hi.z, hi.w};
+  unsigned low[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    low[e] = pack2(x[2 * e] - __uint_as_float(h[e] << 16), x[2 * e + 1] - __uint_as_float(h[e] & 0xFFFF0000u));
+  return make_uint4(low[0], low[1], low[2], low[3]);
+}
+
 // Position of 16-byte chunk c of row r in a 128-byte-swizzled box of 32 rows.
 __device__ __forceinline__ int swizzled(int r, int c) { return r * 128 + (((c ^ r) & 7) << 4); }
 
@@ -313,6 +326,34 @@ struct ListCursor {
     value = values != nullptr && k < K ? values[k] : 0.0f;
   }
 };
+
+// Where the lists of all rows reach `col`, and the first column there: each of the 128 epilogue threads takes two
+// rows, whose searches go on side by side.  (Every warp on its own, its lanes one row after the other, took
+// longer than a tile of 64 hidden columns with 256 rows.)
+__device__ __forceinline__ void seek_rows(const int* list_id, int K, const int* row_no, int rows, int col, int2* cursors) {
+  constexpr int kEach = kFewRows / 128;
+  const int t0 = threadIdx.x - 64;
+  const int* ids[kEach];
+  int lo[kEach], id[kEach];
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    ids[j] = list_id + static_cast<long long>(row_no[min(t0 + j * 128, rows - 1)]) * K;
+    lo[j] = 0;
+  }
+  int top = 1;
+  while (2 * top <= K) top *= 2;
+  for (int step = top; step > 0; step /= 2) {
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) id[j] = ids[j][min(lo[j] + step, K) - 1];
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) lo[j] += lo[j] + step <= K && id[j] < col ? step : 0;
+  }
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) id[j] = ids[j][min(lo[j], K - 1)];
+#pragma unroll
+  for (int j = 0; j < kEach; ++j)
+    if (t0 + j * 128 < rows) cursors[t0 + j * 128] = make_int2(lo[j], lo[j] < K ? id[j] : INT_MAX);
+}
 
 // A row's coefficients of the logits' gradient: {it log2 e, lse log2 e, A, C} of A exp(it l - lse) - C.
 __device__ __forceinline__ float4 row_coefficients(const HeadLossState& s, const float* g, int r) {
@@ -393,7 +434,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW
   const int stage_bytes = sb.a + sb.b;
   const int stages = a.stages;
   uint8_t* sOut = smem + stages * stage_bytes;
-  uint8_t* state = sOut + out_bytes_of(MODE, FEW);
+  uint8_t* state = sOut + out_bytes_of(MODE, FEW, a.kept);
   uint64_t* full = reinterpret_cast<uint64_t*>(state + (FEW && MODE != kProd ? kStateBytes : 0));
   uint64_t* empty = full + kMaxStages;
   uint64_t* tfull = empty + kMaxStages;
@@ -566,6 +607,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW
     };
     int acc = 0, staged = 0;
     uint32_t acc_phase = 0;
+    bool gave_up = false;
     if (FEW && MODE != kProd) {
       for (int t = threadIdx.x - 64; t < kFewRows; t += 128) {
         const int o = t < rows ? a.row_of[t] : -1;
@@ -629,12 +671,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW
       bool live = false;
       if (FEW && MODE != kProd) {
         // every row's place in its list, for this warp's vocabulary columns
-        for (int t = lane; t < rows; t += 32) {
-          cur.ids = a.list_id + static_cast<long long>(row_no[t]) * a.K;
-          cur.values = nullptr;
-          cur.K = a.K;
-          cur.seek(0, a.v0 + m0);
-          cursors[t] = make_int2(cur.k, cur.next);
+        const int first = a.v0 + m0;
+        if (a.K == 1) {
+          for (int t = lane; t < rows; t += 32) {
+            const int id = a.list_id[row_no[t]];
+            cursors[t] = id < first ? make_int2(1, INT_MAX) : make_int2(0, id);
+          }
+        } else {
+          int2* found = cursors + (4 - quarter + (i & 1)) * kFewRows;   // of this CTA's first column; in turn
+          seek_rows(a.list_id, a.K, row_no, rows, a.v0 + it.m0 + rank * held, found);
+          named_barrier(1, 128);
+          if (gave_up) continue;
+          for (int t = lane; t < rows; t += 32) {
+            int2 f = found[t];
+            while (f.y < first) {
+              ++f.x;
+              f.y = f.x < a.K ? a.list_id[static_cast<long long>(row_no[t]) * a.K + f.x] : INT_MAX;
+            }
+            cursors[t] = f;
+          }
         }
         __syncwarp();
       } else if (MODE != kProd) {
@@ -660,7 +715,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW
       }
       if (!empty_sum) {
         const bool ok = __all_sync(0xffffffffu, mbar_wait(&tfull[acc], acc_phase, a.status, kErrEpilogueWait));
-        if (!ok) break;
+        if (!ok) {
+          gave_up = true;
+          if (FEW && MODE != kProd && a.K > 1) continue;   // the other warps still wait for this one above
+          break;
+        }
         tc_fence_after();
       }
       const uint32_t t_acc = tmem + lane_base + acc * kBN;
@@ -696,6 +755,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW
           float x[32];
           tmem_ld32(t_acc + t0, x);
           if (MODE == kStats) {
+            if (a.kept) {
+              // lanes outside the vocabulary are cut off by the map: a warp's columns are its own (see lane_slot)
+              uint8_t* box = next_box(staged);
+              spill_block(box, x);
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                tma_store_2d(&maps.out0, box, t0, m0);
+                bulk_commit();
+              }
+              ++staged;
+            }
 #pragma unroll
             for (int j = 0; j < 32; ++j)
               if (!on) x[j] = -INFINITY;
@@ -706,7 +777,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW
               const float p = reduce_columns(y, [](float u, float v) { return u + v; });
               plains[t] += p;
             }
-            listed(x, t, sOut + quarter * kOutBytes, [&](float* at, long long k) {
+            listed(x, t, sOut + (a.kept ? kOutTotal : 0) + quarter * kOutBytes, [&](float* at, long long k) {
               a.list_logit[k] = *at;
               *at = -INFINITY;
             });
@@ -760,14 +831,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW
                                          pack2(x[8 * q + 4], x[8 * q + 5]), pack2(x[8 * q + 6], x[8 * q + 7]));
               *reinterpret_cast<uint4*>(box + swizzled(lane, (c & 1) * 4 + q)) = on ? v : make_uint4(0, 0, 0, 0);
               if (a.lo > 0) {
-                const unsigned hi[4] = {v.x, v.y, v.z, v.w};
-                unsigned low[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  low[e] = pack2(x[8 * q + 2 * e] - __uint_as_float(hi[e] << 16),
-                                 x[8 * q + 2 * e + 1] - __uint_as_float(hi[e] & 0xFFFF0000u));
-                *reinterpret_cast<uint4*>(box + kOutBytes + swizzled(lane, (c & 1) * 4 + q)) =
-                    on ? make_uint4(low[0], low[1], low[2], low[3]) : make_uint4(0, 0, 0, 0);
+                const uint4 low = rounded_off(x + 8 * q, v);
+                *reinterpret_cast<uint4*>(box + kOutBytes + swizzled(lane, (c & 1) * 4 + q)) = on ? low : make_uint4(0, 0, 0, 0);
               }
             }
             if (c & 1) {
@@ -1330,6 +1395,78 @@ __global__ void __launch_bounds__(128) grad_rows_kernel(const HeadLossState s, c
     if (s.list_id[base + k] != INT_MAX) g.list_grad[base + k] = listed_gradient(s, g.g, r, base + k);
 }
 
+// The logits' gradient of a piece from kept logits: [V, kept pitch] fp32 to [piece, pitch] bf16 (with its second
+// half).  A thread has eight rows, whose inputs it holds, and goes over the vocabulary.  One pass of
+// memory: 6 bytes a logit, 8 with the second half.
+__global__ void __launch_bounds__(256) kept_grad_kernel(const HeadLossState s, const HeadGradArgs g, int kept_pitch, int pitch,
+                                                        int lo, int v0, int cols) {
+  pdl_trigger();
+  pdl_wait();
+  const int rows = *s.count;
+  const int groups = (rows + 63) / 64 * 8;          // of eight rows; the products read whole blocks of 64
+  if (groups == 0) return;
+  const int per = 256 / groups, group = threadIdx.x % groups, first = threadIdx.x / groups;
+  if (first >= per) return;
+  const int t0 = group * 8;
+  float4 coef[8];
+  int id[8];
+  float value[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int r = t0 + e < rows ? s.row_of[t0 + e] : -1;
+    coef[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    id[e] = -1;
+    value[e] = 0.0f;
+    if (r >= 0) {
+      coef[e] = row_coefficients(s, g.g, r);
+      if (s.K == 1) {
+        id[e] = s.list_id[r] - v0;
+        value[e] = listed_gradient(s, g.g, r, r);
+      }
+    }
+  }
+  const int end = min((cols + kBK - 1) / kBK * kBK, g.piece);   // zeros behind the vocabulary, up to its last block
+  for (int v = blockIdx.x * per + first; v < end; v += gridDim.x * per) {
+    float x[8];
+    if (v < cols && t0 < rows) {
+      const float4* src = reinterpret_cast<const float4*>(g.kept + static_cast<long long>(v0 + v) * kept_pitch + t0);
+      const float4 u = __ldcs(src), w = __ldcs(src + 1);
+      x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+      x[4] = w.x; x[5] = w.y; x[6] = w.z; x[7] = w.w;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      // rows behind the last: whatever the memory held
+      x[e] = v < cols && t0 + e < rows ? coef[e].z * ex2(fmaf(x[e], coef[e].x, -coef[e].y)) - coef[e].w : 0.0f;
+      if (v == id[e]) x[e] = value[e];
+    }
+    const uint4 hi = make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7]));
+    __nv_bfloat16* dst = g.dl + static_cast<long long>(v) * pitch + t0;
+    *reinterpret_cast<uint4*>(dst) = hi;
+    if (lo > 0) *reinterpret_cast<uint4*>(dst + lo) = rounded_off(x, hi);
+  }
+}
+
+// Lists of several columns: their gradients, in place of what the pass above left there (one warp a row).
+__global__ void __launch_bounds__(128) kept_listed_kernel(const HeadLossState s, const HeadGradArgs g, int pitch, int lo, int v0,
+                                                          int cols) {
+  pdl_trigger();
+  pdl_wait();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, m = blockIdx.x * 4 + warp;
+  if (m >= *s.count) return;
+  const int r = s.row_of[m];
+  const long long base = static_cast<long long>(r) * s.K;
+  for (int k = lane; k < s.K; k += 32) {
+    const int id = s.list_id[base + k];
+    if (id < v0 || id >= v0 + cols) continue;
+    const float x = listed_gradient(s, g.g, r, base + k);
+    const __nv_bfloat16 hi = __float2bfloat16_rn(x);
+    __nv_bfloat16* dst = g.dl + static_cast<long long>(id - v0) * pitch + m;
+    *dst = hi;
+    if (lo > 0) dst[lo] = __float2bfloat16_rn(x - __bfloat162float(hi));
+  }
+}
+
 __global__ void __launch_bounds__(128) hidden_grad_kernel(const HeadLossState s, const HeadGradArgs g) {
   pdl_trigger();
   pdl_wait();
@@ -1420,7 +1557,7 @@ cudaError_t launch_gemm(const Maps& maps, GemmArgs a, int max_items, cudaStream_
     if (e != cudaSuccess) return e;
     if (dev < 64) set[dev] = true;
   }
-  const int rest = out_bytes_of(MODE, FEW) + (FEW && MODE != kProd ? kStateBytes : 0) + kBarBytes;
+  const int rest = out_bytes_of(MODE, FEW, a.kept) + (FEW && MODE != kProd ? kStateBytes : 0) + kBarBytes;
   const StageBytes sb = stage_bytes_of(MODE, FEW, a);
   a.stages = std::min(kMaxStages, (kSmemMost - rest) / (sb.a + sb.b));
   const int smem = 1024 + a.stages * (sb.a + sb.b) + rest;
@@ -1445,9 +1582,19 @@ GemmArgs base_args(const HeadLossState& s) {
 
 }  // namespace
 
+// Row pitch of the logits that the forward pass keeps for a backward pass, 0 where that recomputes them.  Few rows
+// of logits are small next to the head: 8 bytes a logit, written and read, for the head's 2 H bytes a column and
+// the products with them.  Kept against recomputed, forward and backward: 192 rows of 3584 and 152064
+// columns 613 / 832 us, 16 rows of 1024 177 / 211 us, 128 rows 248 / 256 us, 256 rows of 512 271 / 250 us;
+// 16 rows of a head that stays in L2 (896 x 32768) the same, 128 rows 91 / 76 us.  At most 256 MB.
+int head_loss_kept(int R, int H, int V) {
+  const int pitch = ceil_div(R, 32) * 32;
+  return few_rows(R) && H >= 8 * R && 2ll * H * V >= (128ll << 20) && 4ll * pitch * V <= (256ll << 20) ? pitch : 0;
+}
+
 // Partial statistics per row: one a warp of the launch, or two a tile of columns.
-int head_loss_vocab_tiles(int R, int V) {
-  return few_rows(R) ? 8 * pairs_for(ceil_div(V, 2 * lane_slot(V, 8))) : 2 * ceil_div(V, kBN);
+int head_loss_vocab_tiles(int R, int V, bool kept) {
+  return few_rows(R) ? 8 * pairs_for(ceil_div(V, 2 * lane_slot(V, kept ? 32 : 8))) : 2 * ceil_div(V, kBN);
 }
 
 // Row pitch or row count of the logits' gradient: [piece][few rows, in two halves up to kSplitRows] or
@@ -1517,7 +1664,11 @@ cudaError_t head_loss_forward_launch(const HeadLossState& s, const HeadStatsScra
   a.part_tiles = p.tiles;
   cudaError_t e;
   if (few) {
-    a.slot = lane_slot(s.V, 8);
+    a.kept = p.kept != nullptr;
+    a.slot = lane_slot(s.V, a.kept ? 32 : 8);
+    const int pitch = head_loss_kept(s.R, s.H, s.V);
+    if (a.kept && !encode(&maps.out0, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, p.kept, s.V, pitch, pitch, 32, 32))
+      return cudaErrorInvalidValue;
     if (!map_bf16(&maps.a0, s.w, s.V, s.H, s.ldw, kBK, a.slot) ||
         !map_bf16(&maps.b0, s.hc, s.rpad, s.H, s.H, kBK, a.bn / 2))
       return cudaErrorInvalidValue;
@@ -1549,8 +1700,9 @@ cudaError_t head_loss_backward_launch(const HeadLossState& s, const HeadGradArgs
   const int slot = lane_slot(std::min(g.piece, s.V), 32), pitch = head_loss_grad_rows(s.R);
   bool ok = true;
   if (few) {
-    ok = map_bf16(&gm.a0, s.w, s.V, s.H, s.ldw, kBK, slot) && map_bf16(&gm.b0, s.hc, s.rpad, s.H, s.H, kBK, base.bn / 2) &&
-         map_bf16(&gm.out0, g.dl, g.piece, pitch, pitch, 64, 32);
+    if (g.kept == nullptr)
+      ok = map_bf16(&gm.a0, s.w, s.V, s.H, s.ldw, kBK, slot) && map_bf16(&gm.b0, s.hc, s.rpad, s.H, s.H, kBK, base.bn / 2) &&
+           map_bf16(&gm.out0, g.dl, g.piece, pitch, pitch, 64, 32);
     if (dh)
       ok = ok && map_bf16(&pm.a0, s.w, s.V, s.H, s.ldw, 64, kBK) &&
            map_bf16(&pm.b0, g.dl, g.piece, pitch, pitch, 64, kBK);
@@ -1573,7 +1725,12 @@ cudaError_t head_loss_backward_launch(const HeadLossState& s, const HeadGradArgs
     GemmArgs a = base;
     a.v0 = v0;
     a.cols = std::min(g.piece, s.V - v0);
-    if (few) {
+    if (g.kept != nullptr) {
+      const int blocks = std::min(8 * device_sms(), ceil_div(a.cols, 8));
+      e = launch_pdl(kept_grad_kernel, dim3(blocks), dim3(256), 0, stream, s, g, head_loss_kept(s.R, s.H, s.V), pitch, a.lo, v0, a.cols);
+      if (e == cudaSuccess && s.K > 1)
+        e = launch_pdl(kept_listed_kernel, dim3(ceil_div(s.R, 4)), dim3(128), 0, stream, s, g, pitch, a.lo, v0, a.cols);
+    } else if (few) {
       a.slot = slot;
       e = launch_gemm<kGrad, true>(gm, a, ceil_div(a.cols, 2 * slot), stream);
       a.slot = kHalf;

@@ -51,11 +51,13 @@ struct HeadStatsScratch {
   float2* part;                // [rpad, tiles] max and sum exp of every vocabulary tile, or of every warp's share
   float* part_sum;             // [rpad, tiles] sum of logits (smoothing > 0) or null
   int tiles;
+  float* kept;                 // [V, head_loss_kept] logits of the compact rows for the backward pass, or null
 };
 
 // Backward scratch and outputs.
 struct HeadGradArgs {
   const float* g;              // [R] upstream gradient
+  const float* kept;           // logits that the forward pass kept, or null
   float4* row_coef;            // [rpad]
   float* list_grad;            // [R, K]
   __nv_bfloat16* dl;           // [rpad, piece] gradient of one piece of the logits, or [piece, few rows]
@@ -66,7 +68,8 @@ struct HeadGradArgs {
   __nv_bfloat16* dw;           // [V, H] contiguous or null
 };
 
-int head_loss_vocab_tiles(int R, int V);                // tiles of the statistics scratch
+int head_loss_kept(int R, int H, int V);                // row pitch of logits kept for the backward pass, or 0
+int head_loss_vocab_tiles(int R, int V, bool kept);     // tiles of the statistics scratch
 int head_loss_grad_rows(int R);                         // rows (or row pitch) of the logits' gradient
 int head_loss_piece(int R, int V);                      // default backward piece
 int head_loss_splits(int R, int H, int piece, int V, bool with_dw);   // parts of the hidden gradient's reduction

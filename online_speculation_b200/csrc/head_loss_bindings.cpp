@@ -103,10 +103,11 @@ osb::HeadLossState make_state(const Tensor& w, int64_t R, int64_t H, int64_t K, 
   return s;
 }
 
-// ids [R] (cross entropy) or [R, K] with teacher logits [R, K].  Returns (loss [R], saved bytes).
-std::tuple<Tensor, Tensor> head_loss_forward(Tensor h, Tensor weight, Tensor ids, OptTensor teacher,
+// ids [R] (cross entropy) or [R, K] with teacher logits [R, K].  Returns (loss [R], saved bytes, kept logits or
+// an undefined tensor).
+std::tuple<Tensor, Tensor, Tensor> head_loss_forward(Tensor h, Tensor weight, Tensor ids, OptTensor teacher,
                                              OptTensor teacher_lse, OptTensor inv_temp, int64_t ignore_index,
-                                             double smoothing, double z_loss, Tensor status) {
+                                             double smoothing, double z_loss, bool keep, Tensor status) {
   check_matrix(h, "h");
   check_matrix(weight, "weight");
   TORCH_CHECK(h.size(1) == weight.size(1) && h.device() == weight.device(), "h and weight differ in width or device");
@@ -146,7 +147,13 @@ std::tuple<Tensor, Tensor> head_loss_forward(Tensor h, Tensor weight, Tensor ids
     }
   }
   osb::HeadStatsScratch p{};
-  p.tiles = osb::head_loss_vocab_tiles(s.R, s.V);
+  Tensor kept;
+  const int kept_pitch = keep ? osb::head_loss_kept(s.R, s.H, s.V) : 0;
+  if (kept_pitch > 0) {
+    kept = device_tensor({s.V, kept_pitch}, torch::kFloat32, h);
+    p.kept = kept.data_ptr<float>();
+  }
+  p.tiles = osb::head_loss_vocab_tiles(s.R, s.V, kept_pitch > 0);
   const long long parts = static_cast<long long>(s.rpad) * p.tiles;
   Carve size{nullptr};
   size.take<float2>(parts);
@@ -161,11 +168,11 @@ std::tuple<Tensor, Tensor> head_loss_forward(Tensor h, Tensor weight, Tensor ids
   const auto stream = at::cuda::getCurrentCUDAStream();
   check(osb::head_loss_rows_launch(s, t, stream), "head loss rows");
   check(osb::head_loss_forward_launch(s, p, stream), "head loss forward");
-  return {loss, saved};
+  return {loss, saved, kept};
 }
 
 // Gradients of sum_r g[r] loss[r]: (dh [R, H] or undefined, dW [V, H] or undefined), bf16.
-std::tuple<OptTensor, OptTensor> head_loss_backward(Tensor saved, Tensor weight, OptTensor inv_temp, Tensor g,
+std::tuple<OptTensor, OptTensor> head_loss_backward(Tensor saved, Tensor kept, Tensor weight, OptTensor inv_temp, Tensor g,
                                                     int64_t K, bool divergence, bool rest_bucket, double smoothing,
                                                     double z_loss, bool need_dh, bool need_dw, int64_t piece,
                                                     Tensor status) {
@@ -183,6 +190,7 @@ std::tuple<OptTensor, OptTensor> head_loss_backward(Tensor saved, Tensor weight,
   bind_state(s, static_cast<char*>(saved.data_ptr()));
   osb::HeadGradArgs a{};
   a.g = g.data_ptr<float>();
+  if (kept.defined()) a.kept = kept.data_ptr<float>();
   if (piece > 0) {
     TORCH_CHECK(piece % 256 == 0, "pieces are multiples of 256 columns");
     a.piece = static_cast<int>(std::min<int64_t>(piece, (V + 255) / 256 * 256));
@@ -220,10 +228,11 @@ std::tuple<OptTensor, OptTensor> head_loss_backward(Tensor saved, Tensor weight,
 struct HeadLossNode : public torch::autograd::Function<HeadLossNode> {
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& h, const Tensor& weight, const Tensor& ids,
                         const OptTensor& teacher, const OptTensor& teacher_lse, const OptTensor& inv_temp,
-                        int64_t ignore_index, double smoothing, double z_loss, int64_t piece, const Tensor& status) {
-    auto [loss, saved] = head_loss_forward(h, weight, ids, teacher, teacher_lse, inv_temp, ignore_index, smoothing,
-                                           z_loss, status);
-    ctx->save_for_backward({saved, weight, given(inv_temp) ? *inv_temp : Tensor(), status});
+                        int64_t ignore_index, double smoothing, double z_loss, int64_t piece, bool keep,
+                        const Tensor& status) {
+    auto [loss, saved, kept] = head_loss_forward(h, weight, ids, teacher, teacher_lse, inv_temp, ignore_index, smoothing,
+                                           z_loss, keep, status);
+    ctx->save_for_backward({saved, weight, given(inv_temp) ? *inv_temp : Tensor(), status, kept});
     ctx->saved_data["k"] = given(teacher) ? ids.size(1) : 1;
     ctx->saved_data["divergence"] = given(teacher);
     ctx->saved_data["rest"] = given(teacher_lse);
@@ -241,10 +250,10 @@ struct HeadLossNode : public torch::autograd::Function<HeadLossNode> {
     OptTensor inv_temp;
     if (saved[2].defined()) inv_temp = saved[2];
     auto& d = ctx->saved_data;
-    auto [dh, dw] = head_loss_backward(saved[0], saved[1], inv_temp, g, d["k"].toInt(), d["divergence"].toBool(),
+    auto [dh, dw] = head_loss_backward(saved[0], saved[4], saved[1], inv_temp, g, d["k"].toInt(), d["divergence"].toBool(),
                                        d["rest"].toBool(), d["smoothing"].toDouble(), d["z"].toDouble(),
                                        ctx->needs_input_grad(0), ctx->needs_input_grad(1), d["piece"].toInt(), saved[3]);
-    torch::autograd::variable_list out(11);
+    torch::autograd::variable_list out(12);
     if (given(dh)) out[0] = *dh;
     if (given(dw)) out[1] = *dw;
     return out;
@@ -254,7 +263,9 @@ struct HeadLossNode : public torch::autograd::Function<HeadLossNode> {
 Tensor head_loss(const Tensor& h, const Tensor& weight, const Tensor& ids, const OptTensor& teacher,
                  const OptTensor& teacher_lse, const OptTensor& inv_temp, int64_t ignore_index, double smoothing,
                  double z_loss, int64_t piece, const Tensor& status) {
-  return HeadLossNode::apply(h, weight, ids, teacher, teacher_lse, inv_temp, ignore_index, smoothing, z_loss, piece,
+  // a piece that the caller chose bounds the memory: nothing is kept
+  const bool keep = piece <= 0 && at::GradMode::is_enabled() && (h.requires_grad() || weight.requires_grad());
+  return HeadLossNode::apply(h, weight, ids, teacher, teacher_lse, inv_temp, ignore_index, smoothing, z_loss, piece, keep,
                              status);
 }
 

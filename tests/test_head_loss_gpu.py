@@ -311,6 +311,79 @@ def test_many_rows_and_pieces(cuda):
             oracle.within(got, want[i], want[i + 1], name)
 
 
+# few rows on a head of 128 MB and more: the backward pass reads the logits that the forward pass left
+KEPT = [(1, 1024, 65537), (30, 1000, 70001), (70, 1024, 65700), (128, 1024, 65800), (130, 1048, 64501), (256, 2048, 33001)]
+
+
+@pytest.mark.parametrize("rows,hidden,vocab", KEPT)
+@pytest.mark.parametrize("listed", [0, 1, 40])
+def test_kept_logits(cuda, rows, hidden, vocab, listed):
+    h, w, t, gen = oracle.make_inputs(rows, hidden, vocab, rows + listed, cuda)
+    drop = (torch.rand(rows, generator=gen) < 0.3).to(cuda)
+    drop[rows // 2] = False
+    g = torch.randn(rows, generator=gen).to(cuda)
+    if listed:
+        it = (0.5 + torch.rand(rows, generator=gen)).to(cuda)
+        ids = torch.randint(0, vocab, (rows, listed), generator=gen).to(cuda)
+        ids[0, 0] = vocab - 1
+        ids[-1, -1] = 0
+        ids[drop] = -1
+        teacher = torch.randn(rows, listed, generator=gen).to(cuda)
+        lse = teacher.logsumexp(1) + 1.0 + math.log(2.0)
+        want = oracle.topk_divergence(h, w, ids, teacher, g, it, lse)
+        call = lambda piece: K.head_topk_divergence(h, w, ids, teacher, inv_temp=it, teacher_lse=lse, piece=piece)
+    else:
+        t[drop] = -100
+        t[rows // 2] = vocab - 1
+        want = oracle.cross_entropy(h, w, t, g, smoothing=0.1, z_loss=1e-3)
+        call = lambda piece: K.head_cross_entropy(h, w, t, label_smoothing=0.1, z_loss=1e-3, piece=piece)
+    h[drop] = math.nan
+    h.requires_grad_()
+    w.requires_grad_()
+    for piece in (None, 16384):
+        loss = call(piece)
+        first = torch.autograd.grad(loss, [h, w], g, retain_graph=True)
+        only = torch.autograd.grad(loss, [h], g)[0]
+        workspace.check_status(cuda)
+        oracle.within(loss.detach(), want[0], want[1], "loss")
+        oracle.within(first[0], want[2], want[3], "dh")
+        oracle.within(first[1], want[4], want[5], "dW")
+        oracle.within(only, want[2], want[3], "dh alone")
+
+
+def test_what_is_kept(cuda):
+    """A step keeps the logits of few rows until its graph goes; without gradients, or with a piece, nothing."""
+    rows, hidden, vocab = 16, 1024, 65792
+    h, w, t, _ = oracle.make_inputs(rows, hidden, vocab, 3, cuda)
+    logits = 4 * 32 * vocab
+
+    def held(piece=None):
+        before = torch.cuda.memory_allocated()
+        loss = K.head_cross_entropy(h, w, t, piece=piece)
+        return torch.cuda.memory_allocated() - before, loss
+
+    assert held()[0] < logits
+    h.requires_grad_()
+    with torch.no_grad():
+        assert held()[0] < logits
+    assert held(256)[0] < logits
+    size, loss = held()
+    assert size >= logits
+    whole = torch.cuda.memory_allocated()
+    loss.sum().backward()
+    h.grad = None
+    del loss
+    assert torch.cuda.memory_allocated() <= whole - logits
+    # two steps at a time have their own
+    t2 = t.flip(0)
+    a, b = K.head_cross_entropy(h, w, t), K.head_cross_entropy(h, w, t2)
+    ga, gb = torch.autograd.grad(a.sum(), [h])[0], torch.autograd.grad(b.sum(), [h])[0]
+    ones = torch.ones(rows, device=cuda)
+    for got, target in ((ga, t), (gb, t2)):
+        want = oracle.cross_entropy(h, w, target, ones)
+        oracle.within(got, want[2], want[3], "dh")
+
+
 def test_two_streams_at_once(cuda):
     """Eager calls in flight on two streams share no scratch."""
     cases = []
