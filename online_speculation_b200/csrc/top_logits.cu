@@ -258,6 +258,12 @@ __device__ __forceinline__ void load_raw(const char* row, int i, Raw<kBf16>& r) 
 }
 
 template <bool kBf16>
+__device__ __forceinline__ void fill_raw(Raw<kBf16>& r) {
+#pragma unroll
+  for (uint4& v : r.v) v = make_uint4(0, 0, 0, 0);
+}
+
+template <bool kBf16>
 __device__ __forceinline__ void unpack(const Raw<kBf16>& r, float (&x)[kPer]) {
   if (kBf16) {
     const unsigned u[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
@@ -303,8 +309,9 @@ struct RunningSum {
   float ref = -3.402823466e38f, raise = -INFINITY, s = 0.0f;
   __device__ __forceinline__ void lift(float top, float c2) {
     if (top > raise) {
-      s *= ex2((ref - top) * c2);
-      ref = top;
+      const float now = fminf(top, 3.402823466e38f);   // +inf adds inf about a finite reference
+      s *= ex2((ref - now) * c2);
+      ref = now;
       raise = top + kRaise / c2;
     }
   }
@@ -320,7 +327,41 @@ struct RunningSum {
   }
 };
 
-// Appends the logits marked in `pass` (bit j: x[j], column col + j).
+// Where x[j] is marked in a word of eight: the even ones in the lower half, as packed compares leave them.
+__device__ constexpr unsigned mark(int j) { return 1u << (j / 2 + 16 * (j % 2)); }
+
+__device__ __forceinline__ float largest(const Raw<false>&, const float (&x)[kPer]) {
+  return fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+}
+
+// The logits that are not at or below the bar (a NaN on either side: marked).
+__device__ __forceinline__ unsigned beyond(const Raw<false>&, const float (&x)[kPer], float bar) {
+  unsigned pass = 0;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j)
+    if (!(x[j] <= bar)) pass |= mark(j);
+  return pass;
+}
+
+// bf16 two at a time; the bar is one of the logits, so its rounding is exact.
+__device__ __forceinline__ __nv_bfloat162 pair_of(unsigned u) { return *reinterpret_cast<const __nv_bfloat162*>(&u); }
+
+__device__ __forceinline__ float largest(const Raw<true>& r, const float (&)[kPer]) {
+  const uint4 v = r.v[0];
+  const __nv_bfloat162 m = __hmax2(__hmax2(pair_of(v.x), pair_of(v.y)), __hmax2(pair_of(v.z), pair_of(v.w)));
+  return fmaxf(__low2float(m), __high2float(m));
+}
+
+__device__ __forceinline__ unsigned beyond(const Raw<true>& r, const float (&)[kPer], float bar) {
+  const __nv_bfloat162 b = __float2bfloat162_rn(bar);
+  const unsigned u[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
+  unsigned pass = 0;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) pass |= __hgtu2_mask(pair_of(u[q]), b) & (mark(2 * q) | mark(2 * q + 1));
+  return pass;
+}
+
+// Appends the logits marked in `pass` (x[j]: column col + j).
 __device__ __forceinline__ void append(Smem& sm, const float (&x)[kPer], int col, unsigned pass) {
   if (pass == 0) return;
   const int mine = __popc(pass);
@@ -332,7 +373,7 @@ __device__ __forceinline__ void append(Smem& sm, const float (&x)[kPer], int col
   uint2* dst = reinterpret_cast<uint2*>(sm.cand) + at;
 #pragma unroll
   for (int j = 0; j < kPer; ++j)
-    if (pass & (1u << j)) *dst++ = make_uint2(col + j, __float_as_uint(x[j]));
+    if (pass & mark(j)) *dst++ = make_uint2(col + j, __float_as_uint(x[j]));
 }
 
 // A row's outputs; cand holds n keys, the k largest among them.
@@ -402,18 +443,14 @@ __global__ void __launch_bounds__(kThreads, kBlocks) top_logits_kernel(const Top
   RunningSum sum;
   float bar = __uint_as_float(0x7FFFFFFFu);      // NaN: no bar yet, everything passes
 
-  auto group = [&](const float (&x)[kPer], int col, bool on) {   // whole warps; x is -inf where not on
-    const float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+  auto group = [&](const Raw<kBf16>& r, int col) {      // whole warps
+    float x[kPer];
+    unpack<kBf16>(r, x);
+    const float top = largest(r, x);
     sum.lift(top, c2);
     sum.add_eight(x, c2);
     // a NaN never shows in a maximum, but stays in the sum
-    if (__any_sync(0xffffffffu, !(top <= bar) || !(sum.s == sum.s))) {
-      unsigned pass = 0;
-#pragma unroll
-      for (int j = 0; j < kPer; ++j)
-        if (!(x[j] <= bar)) pass |= 1u << j;
-      append(sm, x, col, on ? pass : 0u);
-    }
+    if (__any_sync(0xffffffffu, !(top <= bar) || !(sum.s == sum.s))) append(sm, x, col, beyond(r, x, bar));
   };
   auto single = [&](int col, bool on) {                 // one column a thread
     float x[kPer] = {0.0f};
@@ -422,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) top_logits_kernel(const Top
       sum.lift(x[0], c2);
       sum.s += ex2((x[0] - sum.ref) * c2);
     }
-    append(sm, x, col, on && !(x[0] <= bar) ? 1u : 0u);
+    append(sm, x, col, on && !(x[0] <= bar) ? mark(0) : 0u);
   };
   auto raise = [&]() {                                  // all threads
     __syncthreads();
@@ -435,43 +472,52 @@ __global__ void __launch_bounds__(kThreads, kBlocks) top_logits_kernel(const Top
       bar = key_float(sm.bar);
     }
   };
-  auto run = [&](int from, int to) {                    // groups [from, to), from a multiple of kThreads
+  auto run = [&](int from, int to) {                    // groups [from, to), multiples of kThreads
+    const int count = (to - from) / kThreads;
     int g = from + tid;
     Raw<kBf16> next[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
-      if (g + u * kThreads < to) load_raw<kBf16>(body, (g + u * kThreads) * kPer, next[u]);
-    for (; g - tid < to; g += kAhead * kThreads) {
+      if (u < count) load_raw<kBf16>(body, (g + u * kThreads) * kPer, next[u]);
+    for (int left = count; left > 0; left -= kAhead, g += kAhead * kThreads) {
       Raw<kBf16> now[kAhead];
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
         now[u] = next[u];
-        const int ahead = g + (kAhead + u) * kThreads;
-        if (ahead < to) load_raw<kBf16>(body, ahead * kPer, next[u]);
+        if (kAhead + u < left) load_raw<kBf16>(body, (g + (kAhead + u) * kThreads) * kPer, next[u]);
       }
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
-        const int at = g + u * kThreads;
-        if (at - tid >= to) break;
-        float x[kPer];
-        unpack<kBf16>(now[u], x);
-        if (at >= to) {
-#pragma unroll
-          for (int j = 0; j < kPer; ++j) x[j] = -INFINITY;
-        }
-        group(x, v0 + at * kPer, at < to);
+        if (u >= left) break;
+        group(now[u], v0 + (g + u * kThreads) * kPer);
       }
     }
   };
+  const int whole = groups / kThreads * kThreads;       // the rest, less than one a thread, comes last
+  auto rest = [&]() {
+    const int g = whole + tid;
+    Raw<kBf16> r;
+    fill_raw<kBf16>(r);
+    if (g < groups) load_raw<kBf16>(body, g * kPer, r);
+    float x[kPer];
+    unpack<kBf16>(r, x);
+    if (g < groups) {
+      sum.lift(largest(r, x), c2);
+      sum.add_eight(x, c2);
+    }
+    append(sm, x, v0 + g * kPer, g < groups ? beyond(r, x, bar) : 0u);
+  };
   single(c0 + tid, tid < head);
   int seen = min(groups, kThreads);
-  run(0, seen);
+  run(0, min(seen, whole));
+  if (whole == 0) rest();
   while (seen < groups) {
     raise();
     // no select just before the end
     const long long grown = static_cast<long long>(seen) * kGrow;
     const int next = grown + grown / 2 >= groups ? groups : static_cast<int>(grown);
-    run(seen, next);
+    run(seen, min(next, whole));
+    if (next == groups) rest();
     seen = next;
   }
   single(tail0 + tid, tail0 + tid < c1);
@@ -498,7 +544,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) top_logits_kernel(const Top
         x[j] = 0.0f;
         if (col < c1) {
           x[j] = load_one(base, kBf16, col);
-          if (bar_key == 0 || order_key(x[j]) > bar_key) pass |= 1u << j;
+          if (bar_key == 0 || order_key(x[j]) > bar_key) pass |= mark(j);
         }
       }
       append(sm, x, col0 + tid * kPer, pass);

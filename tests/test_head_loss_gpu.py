@@ -274,6 +274,24 @@ def test_top_logits_nan_and_signed_zero(cuda):
     assert math.copysign(1, float(values[1, 0])) == -1 and bool(lse[0].isnan())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [300, 10007, 200001])
+def test_top_logits_extremes(cuda, dtype, vocab):
+    """Infinities and the type's lowest value: columns and logsumexp as in 64 bits."""
+    lowest = torch.finfo(dtype).min
+    x = torch.randn(6, vocab, generator=torch.Generator().manual_seed(vocab)).to(dtype)
+    x[0, vocab // 3] = math.inf
+    x[1, [5, vocab - 1]] = math.inf
+    x[2] = -math.inf
+    x[3] = lowest
+    x[4, 100:] = lowest
+    x[5, : vocab - 1] = -math.inf
+    values, ids, lse = K.top_logits(x.to(cuda), 7)
+    v, i, s = _top_reference(x, 7)
+    assert torch.equal(ids.cpu().long(), i) and torch.equal(values.cpu(), v)
+    torch.testing.assert_close(lse.cpu().double(), s, rtol=2.0 ** -22, atol=2.0 ** -17)
+
+
 def test_teacher_to_student(cuda):
     """Teacher logits are listed and kept; the student's head trains on them and on hard labels."""
     rows, hidden, vocab, k = 70, 256, 3000, 32
