@@ -1396,7 +1396,9 @@ __global__ void __launch_bounds__(128) grad_rows_kernel(const HeadLossState s, c
 // The logits' gradient of a piece from kept logits: [V, kept pitch] fp32 to [piece, pitch] bf16 (with its second
 // half).  A thread has eight rows, whose inputs it holds, and goes over the vocabulary.  One pass of
 // memory: 6 bytes a logit, 8 with the second half.
-__global__ void __launch_bounds__(256) kept_grad_kernel(const HeadLossState s, const HeadGradArgs g, int kept_pitch, int pitch,
+constexpr int kKeptAhead = 4;                       // logits of a row in flight a thread
+
+__global__ void __launch_bounds__(256, 2) kept_grad_kernel(const HeadLossState s, const HeadGradArgs g, int kept_pitch, int pitch,
                                                         int lo, int v0, int cols) {
   pdl_trigger();
   pdl_wait();
@@ -1424,24 +1426,34 @@ __global__ void __launch_bounds__(256) kept_grad_kernel(const HeadLossState s, c
     }
   }
   const int end = min((cols + kBK - 1) / kBK * kBK, g.piece);   // zeros behind the vocabulary, up to its last block
-  for (int v = blockIdx.x * per + first; v < end; v += gridDim.x * per) {
-    float x[8];
-    if (v < cols && t0 < rows) {
-      const float4* src = reinterpret_cast<const float4*>(g.kept + static_cast<long long>(v0 + v) * kept_pitch + t0);
-      const float4 u = __ldcs(src), w = __ldcs(src + 1);
-      x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
-      x[4] = w.x; x[5] = w.y; x[6] = w.z; x[7] = w.w;
+  const int step = gridDim.x * per;
+  for (int at = blockIdx.x * per + first; at < end; at += kKeptAhead * step) {
+    float4 in[kKeptAhead][2];
+#pragma unroll
+    for (int u = 0; u < kKeptAhead; ++u) {
+      const int v = at + u * step;
+      if (v < cols && t0 < rows) {
+        const float4* src = reinterpret_cast<const float4*>(g.kept + static_cast<long long>(v0 + v) * kept_pitch + t0);
+        in[u][0] = __ldcs(src);
+        in[u][1] = __ldcs(src + 1);
+      }
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      // rows behind the last: whatever the memory held
-      x[e] = v < cols && t0 + e < rows ? coef[e].z * ex2(fmaf(x[e], coef[e].x, -coef[e].y)) - coef[e].w : 0.0f;
-      if (v == id[e]) x[e] = value[e];
+    for (int u = 0; u < kKeptAhead; ++u) {
+      const int v = at + u * step;
+      if (v >= end) break;
+      float x[8] = {in[u][0].x, in[u][0].y, in[u][0].z, in[u][0].w, in[u][1].x, in[u][1].y, in[u][1].z, in[u][1].w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        // rows behind the last: whatever the memory held
+        x[e] = v < cols && t0 + e < rows ? coef[e].z * ex2(fmaf(x[e], coef[e].x, -coef[e].y)) - coef[e].w : 0.0f;
+        if (v == id[e]) x[e] = value[e];
+      }
+      const uint4 hi = make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7]));
+      __nv_bfloat16* dst = g.dl + static_cast<long long>(v) * pitch + t0;
+      *reinterpret_cast<uint4*>(dst) = hi;
+      if (lo > 0) *reinterpret_cast<uint4*>(dst + lo) = rounded_off(x, hi);
     }
-    const uint4 hi = make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7]));
-    __nv_bfloat16* dst = g.dl + static_cast<long long>(v) * pitch + t0;
-    *reinterpret_cast<uint4*>(dst) = hi;
-    if (lo > 0) *reinterpret_cast<uint4*>(dst + lo) = rounded_off(x, hi);
   }
 }
 
@@ -1502,6 +1514,7 @@ __global__ void __launch_bounds__(128) hidden_grad_kernel(const HeadLossState s,
         x[2 * e + 1] = fmaf(lost[k], __uint_as_float(u[e] & 0xFFFF0000u), x[2 * e + 1]);
       }
     }
+#pragma unroll 4
     for (int q = 0; q < g.splits; ++q) {
       const float4* src = reinterpret_cast<const float4*>(
           g.dh_part + (static_cast<long long>(q) * s.rpad + m) * s.H + i * 8);
@@ -1749,7 +1762,7 @@ cudaError_t head_loss_backward_launch(const HeadLossState& s, const HeadGradArgs
     a.v0 = v0;
     a.cols = std::min(g.piece, s.V - v0);
     if (g.kept != nullptr) {
-      const int blocks = std::min(8 * device_sms(), ceil_div(a.cols, 8));
+      const int blocks = std::min(2 * device_sms(), ceil_div(a.cols, 8));
       e = launch_pdl(kept_grad_kernel, dim3(blocks), dim3(256), 0, stream, s, g, head_loss_kept(s.R, s.H, s.V), pitch, a.lo, v0, a.cols);
       if (e == cudaSuccess && s.K > 1)
         e = launch_pdl(kept_listed_kernel, dim3(ceil_div(s.R, 4)), dim3(128), 0, stream, s, g, pitch, a.lo, v0, a.cols);

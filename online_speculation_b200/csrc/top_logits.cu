@@ -80,12 +80,13 @@ __device__ __forceinline__ void make_keys(Smem& sm, int n) {
   if (threadIdx.x == 0) sm.keyed = n;
 }
 
-// Finds in sm.hist, from the highest bin down, the bin that holds the need-th entry: sm.bin, its
-// entries sm.in_bin and those above it sm.above.  All threads call it, after a barrier; ends in one.
-__device__ __forceinline__ void find_bin(Smem& sm, int need) {
+// This thread's bins, from the highest down: their entries, and those in higher bins than its first.  All threads
+// call it, after a barrier.
+constexpr int kMine = kBins / kThreads;
+
+__device__ __forceinline__ int scan_bins(Smem& sm, int (&own)[kMine]) {
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  constexpr int kMine = kBins / kThreads;
-  int own[kMine], tot = 0;
+  int tot = 0;
 #pragma unroll
   for (int j = 0; j < kMine; ++j) {
     own[j] = sm.hist[kBins - 1 - (tid * kMine + j)];
@@ -102,21 +103,72 @@ __device__ __forceinline__ void find_bin(Smem& sm, int need) {
   int before = incl - tot;
 #pragma unroll
   for (int q = 0; q < kWarps; ++q) before += q < warp ? sm.warp_tot[q] : 0;
+  return before;
+}
+
+// Finds in sm.hist, from the highest bin down, the bin that holds the need-th entry: sm.bin, its
+// entries sm.in_bin and those above it sm.above.  All threads call it, after a barrier; ends in one.
+__device__ __forceinline__ void find_bin(Smem& sm, int need) {
+  int own[kMine];
+  int before = scan_bins(sm, own);
 #pragma unroll
   for (int j = 0; j < kMine; ++j) {
     if (before < need && before + own[j] >= need) {
-      sm.bin = kBins - 1 - (tid * kMine + j);
+      sm.bin = kBins - 1 - (static_cast<int>(threadIdx.x) * kMine + j);
       sm.above = before;
       sm.in_bin = own[j];
     }
     before += own[j];
   }
-  if (tid == 0) sm.count = 0;
+  if (threadIdx.x == 0) sm.count = 0;
   __syncthreads();
 }
 
 __device__ __forceinline__ void clear_bins(Smem& sm) {
   for (int i = threadIdx.x; i < kBins / 4; i += kThreads) reinterpret_cast<int4*>(sm.hist)[i] = make_int4(0, 0, 0, 0);
+}
+
+// Bins that rise with the logit, linear over the range of the candidates.
+struct LinearBins {
+  float lo, scale;
+  __device__ __forceinline__ bool usable() const { return scale > 0.0f && scale < INFINITY; }
+  // NaN and +inf in the last bin, -inf and everything far below in the first
+  __device__ __forceinline__ int of(unsigned long long key) const {
+    const float x = key_float(static_cast<unsigned>(key >> 32));
+    if (!(x < INFINITY)) return kBins - 1;
+    return static_cast<int>(fminf(fmaxf((x - lo) * scale, 0.0f), static_cast<float>(kBins - 1)));
+  }
+};
+
+// For the keys cand[0 .. n); leaves the histogram cleared.  All threads call it; ends in a barrier.
+__device__ __forceinline__ LinearBins linear_bins(Smem& sm, int n) {
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  float lo = INFINITY, hi = -INFINITY;
+  for (int i = tid; i < n; i += kThreads) {
+    const float x = key_float(static_cast<unsigned>(sm.cand[i] >> 32));
+    if (fabsf(x) < INFINITY) {
+      lo = fminf(lo, x);
+      hi = fmaxf(hi, x);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  }
+  if (lane == 0) {
+    sm.lo[warp] = lo;
+    sm.hi[warp] = hi;
+  }
+  clear_bins(sm);
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < kWarps; ++q) {
+    lo = fminf(lo, sm.lo[q]);
+    hi = fmaxf(hi, sm.hi[q]);
+  }
+  lo = fmaxf(lo, hi - kSpread);
+  return {lo, (kBins - 1) / (hi - lo)};
 }
 
 // Moves the entries that keep(key) holds for to the front, in rounds: a round's entries are read
@@ -146,47 +198,16 @@ __device__ __forceinline__ void compact(Smem& sm, int n, Keep keep) {
 // equally full, where the leading bits of a float crowd into a few); what that leaves too many
 // of, many equal logits or far outliers, is cut by radix digits of the key from the top.
 __device__ int narrow(Smem& sm, int n, int k, int limit) {
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int tid = threadIdx.x, lane = tid % 32;
   if (n <= limit) return n;
-  float lo = INFINITY, hi = -INFINITY;
-  for (int i = tid; i < n; i += kThreads) {
-    const float x = key_float(static_cast<unsigned>(sm.cand[i] >> 32));
-    if (fabsf(x) < INFINITY) {
-      lo = fminf(lo, x);
-      hi = fmaxf(hi, x);
-    }
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-  }
-  if (lane == 0) {
-    sm.lo[warp] = lo;
-    sm.hi[warp] = hi;
-  }
-  clear_bins(sm);
   if (tid == 0) sm.bar = 0xFFFFFFFFu;
-  __syncthreads();
-#pragma unroll
-  for (int q = 0; q < kWarps; ++q) {
-    lo = fminf(lo, sm.lo[q]);
-    hi = fmaxf(hi, sm.hi[q]);
-  }
-  lo = fmaxf(lo, hi - kSpread);
-  const float scale = (kBins - 1) / (hi - lo);
-  if (scale > 0.0f && scale < INFINITY) {
-    // rising in x: NaN and +inf in the last bin, -inf and everything far below in the first
-    auto bin_of = [&](unsigned long long key) {
-      const float x = key_float(static_cast<unsigned>(key >> 32));
-      if (!(x < INFINITY)) return kBins - 1;
-      return static_cast<int>(fminf(fmaxf((x - lo) * scale, 0.0f), static_cast<float>(kBins - 1)));
-    };
-    for (int i = tid; i < n; i += kThreads) atomicAdd(&sm.hist[bin_of(sm.cand[i])], 1);
+  const LinearBins bins = linear_bins(sm, n);
+  if (bins.usable()) {
+    for (int i = tid; i < n; i += kThreads) atomicAdd(&sm.hist[bins.of(sm.cand[i])], 1);
     __syncthreads();
     find_bin(sm, k);
     const int edge = sm.bin;
-    compact(sm, n, [&](unsigned long long key) { return bin_of(key) >= edge; });
+    compact(sm, n, [&](unsigned long long key) { return bins.of(key) >= edge; });
     n = sm.count;
   }
   if (n > limit) {
@@ -222,14 +243,60 @@ __device__ int narrow(Smem& sm, int n, int k, int limit) {
   return kept;
 }
 
-// Calls put(key, rank) for the k largest of cand[0 .. n), n >= k or all of them.
+// Sorts the keys cand[0 .. n), n at most kCap / 2, descending; ends in a barrier.  A counting sort over linear bins,
+// then compares within a bin.
+__device__ __noinline__ void sort_keys(int n) {
+  extern __shared__ __align__(16) uint8_t raw[];
+  Smem& sm = *reinterpret_cast<Smem*>(raw);
+  static_assert(2 * rank_limit(kTopLogitsMax) <= kCap, "room for the sorted keys");
+  const int tid = threadIdx.x;
+  unsigned long long* sorted = sm.cand + kCap / 2;
+  __syncthreads();
+  LinearBins bins = linear_bins(sm, n);
+  if (!bins.usable()) bins = {0.0f, 0.0f};               // no spread: the first bin, infinities and NaN in the last
+  for (int i = tid; i < n; i += kThreads) atomicAdd(&sm.hist[bins.of(sm.cand[i])], 1);
+  __syncthreads();
+  int own[kMine];
+  int before = scan_bins(sm, own);
+#pragma unroll
+  for (int j = 0; j < kMine; ++j) {                      // where a bin's keys begin
+    sm.hist[kBins - 1 - (tid * kMine + j)] = before;
+    before += own[j];
+  }
+  __syncthreads();
+  for (int i = tid; i < n; i += kThreads) {
+    const unsigned long long key = sm.cand[i];
+    sorted[atomicAdd(&sm.hist[bins.of(key)], 1)] = key;  // and, when all are placed, where they end
+  }
+  __syncthreads();
+  for (int i = tid; i < n; i += kThreads) {
+    const unsigned long long key = sorted[i];
+    const int bin = bins.of(key);
+    const int first = bin + 1 < kBins ? sm.hist[bin + 1] : 0, end = sm.hist[bin];
+    int rank = first;
+    for (int j = first; j < end; ++j) rank += sorted[j] > key;
+    sm.cand[rank] = key;
+  }
+  __syncthreads();
+}
+
+// Calls put(key, rank) for the k largest of cand[0 .. n), n at most rank_limit(k), n >= k or all of them.
+// More of them than threads are sorted: comparing all with all grows with k^2 (1021 rows of 151937, k 256: 142 us for
+// 135 us).  Fewer are compared, all with all: the sort's barriers take longer (4 rows of 152064, k 16: 18.5 us
+// for 15.8 us).
 template <typename Put>
 __device__ void rank_top(Smem& sm, int n, int k, Put put) {
-  if (threadIdx.x == 0 && (n & 1)) sm.cand[n] = 0ull;   // below every key
+  const int tid = threadIdx.x;
+  if (n > kThreads) {
+    sort_keys(n);
+    for (int i = tid; i < min(n, k); i += kThreads) put(sm.cand[i], i);
+    return;
+  }
+  if (tid == 0 && (n & 1)) sm.cand[n] = 0ull;            // below every key
   __syncthreads();
   const ulonglong2* pairs = reinterpret_cast<const ulonglong2*>(sm.cand);
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const unsigned long long key = sm.cand[i];
+  if (tid < n) {
+    const unsigned long long key = sm.cand[tid];
     int rank = 0;
 #pragma unroll 8
     for (int j = 0; j < (n + 1) / 2; ++j) {
