@@ -1618,14 +1618,15 @@ GemmArgs base_args(const HeadLossState& s) {
 
 }  // namespace
 
-// Row pitch of the logits that the forward pass keeps for a backward pass, 0 where that recomputes them.  Few rows
-// of logits are small next to the head: 8 bytes a logit, written and read, for the head's 2 H bytes a column and
-// the products with them.  Kept against recomputed, forward and backward: 192 rows of 3584 and 152064
-// columns 613 / 832 us, 16 rows of 1024 177 / 211 us, 128 rows 248 / 256 us, 256 rows of 512 271 / 250 us;
-// 16 rows of a head that stays in L2 (896 x 32768) the same, 128 rows 91 / 76 us.  At most 256 MB.
+// Row pitch of the logits that the forward pass keeps for a backward pass, 0 where that recomputes them.  A logit
+// kept is 8 bytes, written and read, and saves the second reading of the head with its products.  Forward and
+// hidden gradient, kept against recomputed: 192 rows of 3584 and 152064 columns 554 / 851 us, 16 rows of 3584
+// 426 / 582 us, 128 rows of 512 174 / 185 us, 256 rows of 64 218 / 215 us; 128 rows of 896 and 32768 columns
+// 75 / 80 us, 64 rows of 512 and 20000 columns 74 / 72 us (one more launch and allocation).  At most 256 MB, and at most
+// twice the head.
 int head_loss_kept(int R, int H, int V) {
   const int pitch = ceil_div(R, 32) * 32;
-  return few_rows(R) && H >= 8 * R && 2ll * H * V >= (128ll << 20) && 4ll * pitch * V <= (256ll << 20) ? pitch : 0;
+  return few_rows(R) && R <= H && V >= 32768 && 4ll * pitch * V <= (256ll << 20) ? pitch : 0;
 }
 
 // Partial statistics per row: one a warp of the launch, or two a tile of columns.

@@ -75,8 +75,8 @@ def head_cross_entropy(h: torch.Tensor, weight: torch.Tensor, targets: torch.Ten
     its row is ignored and ``workspace.check_status`` reports it.  Gradients are bf16, summed in
     fp32.  ``piece`` (a multiple of 256): vocabulary columns the backward pass works on at a
     time; its scratch is ``2 R piece`` bytes (256 MB without it).  Without it, a step of at most 256
-    rows on a head of 128 MB or more that is wide for them (H at least 8 R) keeps its logits for the
-    backward pass, ``4 R V`` bytes up to 256 MB, instead of computing them twice.
+    (and H) rows on 32768 columns or more keeps its logits for the backward pass, ``4 R V`` bytes up to
+    256 MB, instead of computing them twice.
 
     A training step that is captured into a CUDA graph takes its gradients with
     ``torch.autograd.grad``; no eager graph of the same leaves may be alive meanwhile.

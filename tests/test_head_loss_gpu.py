@@ -329,8 +329,9 @@ def test_many_rows_and_pieces(cuda):
             oracle.within(got, want[i], want[i + 1], name)
 
 
-# few rows on a head of 128 MB and more: the backward pass reads the logits that the forward pass left
-KEPT = [(1, 1024, 65537), (30, 1000, 70001), (70, 1024, 65700), (128, 1024, 65800), (130, 1048, 64501), (256, 2048, 33001)]
+# few rows on many columns: the backward pass reads the logits that the forward pass left
+KEPT = [(3, 8, 32768), (200, 256, 40000), (255, 264, 32769), (1, 1024, 65537), (30, 1000, 70001), (70, 1024, 65700),
+        (128, 1024, 65800), (130, 1048, 64501), (256, 2048, 33001)]
 
 
 @pytest.mark.parametrize("rows,hidden,vocab", KEPT)
@@ -509,3 +510,117 @@ def test_side_stream_and_graph_replay(cuda):
             for got, j in zip(out, (0, 2, 4)):
                 oracle.within(got, want[j], want[j + 1], (seed, j))
     workspace.check_status(cuda)
+
+
+def test_distillation_step_in_a_graph(cuda):
+    """Teacher logits listed, student trained on them (kept logits), in one captured step next to an eager one."""
+    rows, hidden, vocab, k = 48, 256, 33000, 20
+    h, w, _, gen = oracle.make_inputs(rows, hidden, vocab, 90, cuda)
+    big = torch.randn(rows, vocab, generator=gen).to(cuda)
+    it = (0.7 + torch.rand(rows, generator=gen)).to(cuda)
+    g = torch.randn(rows, generator=gen).to(cuda)
+    h.requires_grad_()
+    w.requires_grad_()
+
+    def step():
+        values, ids, lse = K.top_logits(big, k, inv_temp=it)
+        loss = K.head_topk_divergence(h, w, ids, values, inv_temp=it, teacher_lse=lse)
+        return (loss.detach(), *torch.autograd.grad(loss, [h, w], g), ids, values, lse)
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        out = step()
+    for seed in (91, 92):
+        nh, nw, _, gen = oracle.make_inputs(rows, hidden, vocab, seed, cuda)
+        with torch.no_grad():
+            h.copy_(nh)
+            w.copy_(nw)
+            big.copy_(3 * torch.randn(rows, vocab, generator=gen).to(cuda))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+        eager = step()
+        torch.cuda.synchronize()
+        want = oracle.topk_divergence(h, w, eager[3], eager[4], g, it, eager[5])
+        for run in (out, eager):
+            for i in range(3):
+                oracle.within(run[i], want[2 * i], want[2 * i + 1], (seed, i))
+        assert all(torch.equal(a, b) for a, b in zip(out, eager))
+    workspace.check_status(cuda)
+
+
+@pytest.mark.parametrize("rows", [40, 300])
+def test_edges_of_the_arguments(cuda, rows):
+    """Targets smoothed away, an ignored index inside the vocabulary, a piece beyond it, inference mode."""
+    h, w, t, gen = oracle.make_inputs(rows, 64, 500, 15, cuda)
+    t[::3] = 7
+    g = torch.randn(rows, generator=gen).to(cuda)
+    want = oracle.cross_entropy(h, w, t, g, ignore_index=7, smoothing=1.0, z_loss=0.5)
+    h.requires_grad_()
+    w.requires_grad_()
+    loss = K.head_cross_entropy(h, w, t, ignore_index=7, label_smoothing=1.0, z_loss=0.5, piece=1 << 30)
+    for got, i in zip((loss.detach(), *_grads(loss, h, w, g)), (0, 2, 4)):
+        oracle.within(got, want[i], want[i + 1], i)
+    with torch.inference_mode():
+        again = K.head_cross_entropy(h, w, t, ignore_index=7, label_smoothing=1.0, z_loss=0.5)
+    assert not again.requires_grad
+    oracle.within(again, want[0], want[1], "loss")
+
+
+def test_offsets_past_32_bits(cuda):
+    """Rows more than 2^31 elements apart, and a head whose rows reach past 2^31 elements."""
+    gen = torch.Generator().manual_seed(1)
+    far = (1 << 31) + 24
+    logits = torch.empty(far + 6000, dtype=torch.bfloat16, device=cuda).as_strided((2, 5000), (far, 1), 3)
+    logits.copy_(torch.randn(2, 5000, generator=gen))
+    values, ids, lse = K.top_logits(logits, 9)
+    v, i, s = _top_reference(logits, 9)
+    assert torch.equal(ids.cpu().long(), i) and torch.equal(values.cpu(), v)
+    torch.testing.assert_close(lse.cpu().double(), s, rtol=2.0 ** -22, atol=2.0 ** -17)
+    del logits
+    vocab, hidden = 140000, 64
+    pitch = 16 * 1025
+    wide = torch.empty(vocab * pitch, dtype=torch.bfloat16, device=cuda).as_strided((vocab, hidden), (pitch, 1))
+    for rows in (20, 300):
+        h, w, t, gen = oracle.make_inputs(rows, hidden, vocab, rows, cuda)
+        wide.copy_(w)
+        t[0] = vocab - 1
+        g = torch.randn(rows, generator=gen).to(cuda)
+        want = oracle.cross_entropy(h, w, t, g)
+        h.requires_grad_()
+        head = wide.detach().requires_grad_()
+        loss = K.head_cross_entropy(h, head, t)
+        for got, i in zip((loss.detach(), *_grads(loss, h, head, g)), (0, 2, 4)):
+            oracle.within(got, want[i], want[i + 1], (rows, i))
+
+
+def test_head_of_more_than_32_bits(cuda):
+    """A contiguous head, and its gradient, of more than 2^31 elements; a few rows of it are looked at."""
+    rows, hidden, vocab = 5, 16384, 133000
+    h = torch.randn(rows, hidden, device=cuda).bfloat16()
+    w = torch.empty(vocab, hidden, dtype=torch.bfloat16, device=cuda).normal_(0, 1 / 128)
+    t = torch.tensor([0, vocab - 1, 70001, 132000, vocab - 1], device=cuda)
+    logits = torch.cat([(h.double() @ w[i:i + 7000].double().t()) for i in range(0, vocab, 7000)], 1)
+    lse = logits.logsumexp(1)
+    dl = (logits - lse[:, None]).exp()
+    dl[torch.arange(rows, device=cuda), t] -= 1
+    dh_want = sum(dl[:, i:i + 7000] @ w[i:i + 7000].double() for i in range(0, vocab, 7000))
+    h.requires_grad_()
+    w.requires_grad_()
+    loss = K.head_cross_entropy(h, w, t)
+    dh, dw = _grads(loss, h, w, torch.ones(rows, device=cuda))
+    hd = h.detach().double()
+    err = 2 * math.sqrt(hidden) * oracle.FP32_HALF * float((hd.abs() @ w[:7000].detach().double().abs().t()).max())
+    want = lse - logits.gather(1, t[:, None])[:, 0]
+    assert float((loss.detach() - want).abs().max()) <= 2 * err + 8 * oracle.FP32_HALF * (float(want.max()) + 1)
+    # half a step of the output, and what the logits' error (relative to p: twice it) does
+    off = oracle.BF16_HALF + 4 * err
+    assert float((dh - dh_want).norm()) <= off * float(dh_want.norm())
+    for part in (slice(0, 300), slice(69900, 70100), slice(vocab - 300, vocab)):
+        dw_want = dl[:, part].t() @ hd
+        assert float((dw[part] - dw_want).norm()) <= off * float(dw_want.norm())
