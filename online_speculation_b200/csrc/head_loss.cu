@@ -35,6 +35,8 @@
 #include "common.cuh"
 #include "head_loss.h"
 
+#include <cuda_fp16.h>
+
 #include <algorithm>
 #include <climits>
 
@@ -66,6 +68,9 @@ constexpr int kStateMax = 0, kStateSum = kStateMax + 4 * kFewRows * 4, kStatePla
 constexpr int kBarBytes = 256;            // barriers and the TMEM address
 constexpr int kSmemMost = 232448 - 1024;               // behind the alignment
 constexpr float kLog2e = 1.4426950408889634f;
+// Kept exponentials are fp16 of 2^15 exp(it (l - the largest of 128 columns)): off by 2^-11 relative down to e^-20 of the
+// largest, by 2^-40 of it below.
+constexpr float kKeptOne = 32768.0f;
 
 enum Mode { kStats = 0, kGrad = 1, kProd = 2 };
 
@@ -95,7 +100,7 @@ struct GemmArgs {
   HeadLossState s;         // rows in columns, grad: coefficients and listed values are formed on the spot
   const float* g;
   const float* inv_temp;   // stats
-  int kept;                // stats with rows in columns: the logits are stored for the backward pass
+  int kept;                // stats: the logits (rows in columns) or their exponentials are stored for the backward pass
   float2* part;
   float* part_sum;
   int part_tiles;
@@ -121,7 +126,7 @@ __host__ __device__ inline StageBytes stage_bytes_of(int mode, bool few, const G
 
 __host__ __device__ inline int out_bytes_of(int mode, bool few, bool kept) {
   if (few && mode == kProd) return 2 * kOutTotal;
-  if (!few) return mode == kStats ? 0 : kOutTotal;
+  if (!few) return mode == kStats && !kept ? 0 : kOutTotal;
   return (mode == kStats && !kept ? 0 : kOutTotal) + kOutTotal / 2;   // a block for listed logits, behind the boxes
 }
 
@@ -863,6 +868,78 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW
             ++staged;
           }
         }
+      } else if (MODE == kStats && a.kept) {
+        // the warp's half of the tile in registers, exponentials about its maximum
+        float x[kBN / 64][32], plain = 0.0f;
+        const int first = it.n0 + set * (kBN / 2);
+        if (m0 < rows) {
+          float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 0; c < kBN / 64; ++c) {
+            const int col = first + c * 32;
+            tmem_ld32(t_acc + set * (kBN / 2) + c * 32, x[c]);
+            if (col + 32 > a.V) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                if (col + j < a.V) plain += x[c][j];
+                else x[c][j] = -INFINITY;
+              }
+            } else if (a.part_sum != nullptr) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) plain += x[c][j];
+            }
+            while (cur.next < min(col + 32, a.V)) {
+              const int at = cur.next - col;
+              float v = 0.0f;
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (j == at) {
+                  v = x[c][j];
+                  x[c][j] = -INFINITY;
+                }
+              a.list_logit[list0 + cur.k] = v;
+              cur.advance();
+            }
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) tops[j & 3] = fmaxf(tops[j & 3], x[c][j]);
+          }
+          const float mx = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+          const float ref = mx == -INFINITY ? 0.0f : mx;
+          const float2 minus = make_float2(-ref, -ref), scale = make_float2(c2, c2), up = make_float2(kKeptOne, kKeptOne);
+          float2 s2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            uint8_t* box = next_box(staged);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              unsigned packed[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float* from = &x[2 * b + q / 4][(q % 4) * 8 + 2 * e];
+                float2 d = mul2(add2(make_float2(from[0], from[1]), minus), scale);
+                d = make_float2(ex2(d.x), ex2(d.y));
+                s2[e & 1] = add2(s2[e & 1], d);
+                d = mul2(d, up);
+                const __half2 h = __floats2half2_rn(d.x, d.y);
+                packed[e] = *reinterpret_cast<const unsigned*>(&h);
+              }
+              *reinterpret_cast<uint4*>(box + swizzled(lane, q)) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&maps.out0, box, first + b * 64, m0);
+              bulk_commit();
+            }
+            ++staged;
+          }
+          if (live) {
+            const long long p = static_cast<long long>(m) * a.part_tiles + 2 * (it.n0 / kBN) + set;
+            a.part[p] = make_float2(mx, (s2[0].x + s2[1].x) + (s2[0].y + s2[1].y));
+            if (a.part_sum != nullptr) a.part_sum[p] = plain;
+          }
+        }
       } else if (MODE == kStats) {
         float mx = -INFINITY, sum = 0.0f, plain = 0.0f;
         const int end = min(a.V, it.n0 + kBN);         // behind the tile's last column
@@ -1433,7 +1510,7 @@ __global__ void __launch_bounds__(256, 2) kept_grad_kernel(const HeadLossState s
     for (int u = 0; u < kKeptAhead; ++u) {
       const int v = at + u * step;
       if (v < cols && t0 < rows) {
-        const float4* src = reinterpret_cast<const float4*>(g.kept + static_cast<long long>(v0 + v) * kept_pitch + t0);
+        const float4* src = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(g.kept) + static_cast<long long>(v0 + v) * kept_pitch + t0);
         in[u][0] = __ldcs(src);
         in[u][1] = __ldcs(src + 1);
       }
@@ -1454,6 +1531,78 @@ __global__ void __launch_bounds__(256, 2) kept_grad_kernel(const HeadLossState s
       *reinterpret_cast<uint4*>(dst) = hi;
       if (lo > 0) *reinterpret_cast<uint4*>(dst + lo) = rounded_off(x, hi);
     }
+  }
+}
+
+// The same from kept exponentials of many rows: [rpad, pitch] fp16 about the maxima of 128 columns to [rpad, piece] bf16.
+// A block takes 8192 columns of a row.
+__global__ void __launch_bounds__(256) kept_scale_kernel(const HeadLossState s, const HeadGradArgs g, const HeadKept k, int v0,
+                                                         int cols) {
+  pdl_trigger();
+  pdl_wait();
+  constexpr int kVecs = 4;
+  const int m = blockIdx.x, rows = *s.count;
+  if (m >= (rows + kBK - 1) / kBK * kBK) return;           // the head gradient's product reads whole blocks of 64
+  const int end = min((cols + kBK - 1) / kBK * kBK, g.piece), begin = blockIdx.y * kVecs * 2048;
+  __nv_bfloat16* dst = g.dl + static_cast<long long>(m) * g.piece;
+  if (m >= rows) {
+    for (int v = begin + threadIdx.x * 8; v < min(end, begin + kVecs * 2048); v += 2048)
+      *reinterpret_cast<uint4*>(dst + v) = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  const __half* src = reinterpret_cast<const __half*>(g.kept) + static_cast<long long>(m) * k.pitch + v0;
+  const float2* part = reinterpret_cast<const float2*>(g.kept + k.part_at) + static_cast<long long>(m) * k.tiles + v0 / 128;
+  uint4 in[kVecs];
+  float ref[kVecs];
+#pragma unroll
+  for (int u = 0; u < kVecs; ++u) {
+    const int v = begin + u * 2048 + threadIdx.x * 8;
+    if (v < cols) {
+      in[u] = __ldcs(reinterpret_cast<const uint4*>(src + v));
+      ref[u] = part[v / 128].x;
+    }
+  }
+  const float4 coef = g.row_coef[m];
+  const long long base = static_cast<long long>(s.row_of[m]) * s.K;
+  // listed columns of this block: from `from` on
+  int from = 0;
+  if (s.K > 1) {
+    int hi = s.K;
+    while (from < hi) {
+      const int mid = (from + hi) >> 1;
+      if (s.list_id[base + mid] < v0 + begin) from = mid + 1; else hi = mid;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kVecs; ++u) {
+    const int v = begin + u * 2048 + threadIdx.x * 8;
+    if (begin + u * 2048 >= end) break;
+    const float scale = coef.z * ex2(fmaf(ref[u], coef.x, -coef.y)) * (1.0f / kKeptOne);
+    const unsigned w[4] = {in[u].x, in[u].y, in[u].z, in[u].w};
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+      x[2 * e] = fmaf(f.x, scale, -coef.w);
+      x[2 * e + 1] = fmaf(f.y, scale, -coef.w);
+    }
+    if (v + 8 > cols) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (v + e >= cols) x[e] = 0.0f;
+    }
+    for (; from < s.K; ++from) {
+      const int at = s.list_id[base + from] - v0 - (begin + u * 2048);
+      if (at >= 2048) break;
+      if (at / 8 == static_cast<int>(threadIdx.x) && at >= 0) {
+        const float value = g.list_grad[base + from];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e == at % 8) x[e] = value;
+      }
+    }
+    if (v < end)
+      *reinterpret_cast<uint4*>(dst + v) = make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7]));
   }
 }
 
@@ -1624,9 +1773,20 @@ GemmArgs base_args(const HeadLossState& s) {
 // 426 / 582 us, 128 rows of 512 174 / 185 us, 256 rows of 64 218 / 215 us; 128 rows of 896 and 32768 columns
 // 75 / 80 us, 64 rows of 512 and 20000 columns 74 / 72 us (one more launch and allocation).  At most 256 MB, and at most
 // twice the head.
-int head_loss_kept(int R, int H, int V) {
-  const int pitch = ceil_div(R, 32) * 32;
-  return few_rows(R) && R <= H && V >= 32768 && 4ll * pitch * V <= (256ll << 20) ? pitch : 0;
+HeadKept head_loss_kept(int R, int H, int V) {
+  HeadKept k{};
+  if (few_rows(R)) {
+    k.pitch = ceil_div(R, 32) * 32;
+    k.bytes = 4ll * k.pitch * V;
+    if (R > H || V < 32768 || k.bytes > (256ll << 20)) return HeadKept{};
+    return k;
+  }
+  const long long rpad = static_cast<long long>(ceil_div(R, kHeadRowPad)) * kHeadRowPad;
+  k.pitch = ceil_div(V, kBN) * kBN;
+  k.tiles = 2 * ceil_div(V, kBN);
+  k.part_at = 2 * rpad * k.pitch;
+  k.bytes = k.part_at + rpad * k.tiles * static_cast<long long>(sizeof(float2));
+  return k.part_at <= (2ll << 30) ? k : HeadKept{};
 }
 
 // Partial statistics per row: one a warp of the launch, or two a tile of columns.
@@ -1703,7 +1863,7 @@ cudaError_t head_loss_forward_launch(const HeadLossState& s, const HeadStatsScra
   if (few) {
     a.kept = p.kept != nullptr;
     a.slot = lane_slot(s.V, a.kept ? 32 : 8);
-    const int pitch = head_loss_kept(s.R, s.H, s.V);
+    const int pitch = head_loss_kept(s.R, s.H, s.V).pitch;
     if (a.kept && !encode(&maps.out0, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, p.kept, s.V, pitch, pitch, 32, 32))
       return cudaErrorInvalidValue;
     if (!map_bf16(&maps.a0, s.w, s.V, s.H, s.ldw, kBK, a.slot) ||
@@ -1713,6 +1873,9 @@ cudaError_t head_loss_forward_launch(const HeadLossState& s, const HeadStatsScra
   } else {
     if (!map_bf16(&maps.a0, s.hc, s.rpad, s.H, s.H, kBK, kHalf) || !map_bf16(&maps.b0, s.w, s.V, s.H, s.ldw, kBK, kHalf))
       return cudaErrorInvalidValue;
+    a.kept = p.kept != nullptr;
+    const int pitch = head_loss_kept(s.R, s.H, s.V).pitch;
+    if (a.kept && !map_bf16(&maps.out0, p.kept, s.rpad, pitch, pitch, 64, 32)) return cudaErrorInvalidValue;   // fp16
     e = launch_gemm<kStats, false>(maps, a, ceil_div(s.R, kBM) * a.tiles_n, stream);
   }
   if (e != cudaSuccess) return e;
@@ -1745,8 +1908,9 @@ cudaError_t head_loss_backward_launch(const HeadLossState& s, const HeadGradArgs
            map_bf16(&pm.b0, g.dl, g.piece, pitch, pitch, 64, kBK);
     if (dw) ok = ok && map_bf16(&pm.a1, g.dl, g.piece, pitch, pitch, kBK, kHalf);
   } else {
-    ok = map_bf16(&gm.a0, s.hc, s.rpad, s.H, s.H, kBK, kHalf) && map_bf16(&gm.b0, s.w, s.V, s.H, s.ldw, kBK, kHalf) &&
-         map_bf16(&gm.out0, g.dl, s.rpad, g.piece, g.piece, 64, 32);
+    if (g.kept == nullptr)
+      ok = map_bf16(&gm.a0, s.hc, s.rpad, s.H, s.H, kBK, kHalf) && map_bf16(&gm.b0, s.w, s.V, s.H, s.ldw, kBK, kHalf) &&
+           map_bf16(&gm.out0, g.dl, s.rpad, g.piece, g.piece, 64, 32);
     if (dh)
       ok = ok && map_bf16(&pm.a0, g.dl, s.rpad, g.piece, g.piece, kBK, kHalf) &&
            map_bf16(&pm.b0, s.w, s.V, s.H, s.ldw, 64, kBK);
@@ -1762,9 +1926,12 @@ cudaError_t head_loss_backward_launch(const HeadLossState& s, const HeadGradArgs
     GemmArgs a = base;
     a.v0 = v0;
     a.cols = std::min(g.piece, s.V - v0);
-    if (g.kept != nullptr) {
+    if (g.kept != nullptr && !few) {
+      e = launch_pdl(kept_scale_kernel, dim3(s.rpad, ceil_div(a.cols, 8192)), dim3(256), 0, stream, s, g,
+                     head_loss_kept(s.R, s.H, s.V), v0, a.cols);
+    } else if (g.kept != nullptr) {
       const int blocks = std::min(2 * device_sms(), ceil_div(a.cols, 8));
-      e = launch_pdl(kept_grad_kernel, dim3(blocks), dim3(256), 0, stream, s, g, head_loss_kept(s.R, s.H, s.V), pitch, a.lo, v0, a.cols);
+      e = launch_pdl(kept_grad_kernel, dim3(blocks), dim3(256), 0, stream, s, g, head_loss_kept(s.R, s.H, s.V).pitch, pitch, a.lo, v0, a.cols);
       if (e == cudaSuccess && s.K > 1)
         e = launch_pdl(kept_listed_kernel, dim3(ceil_div(s.R, 4)), dim3(128), 0, stream, s, g, pitch, a.lo, v0, a.cols);
     } else if (few) {

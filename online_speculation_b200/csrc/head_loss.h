@@ -51,13 +51,14 @@ struct HeadStatsScratch {
   float2* part;                // [rpad, tiles] max and sum exp of every vocabulary tile, or of every warp's share
   float* part_sum;             // [rpad, tiles] sum of logits (smoothing > 0) or null
   int tiles;
-  float* kept;                 // [V, head_loss_kept] logits of the compact rows for the backward pass, or null
+  char* kept;                  // what the backward pass needs of the logits (HeadKept), or null; `part` lies in it
+                               // for many rows
 };
 
 // Backward scratch and outputs.
 struct HeadGradArgs {
   const float* g;              // [R] upstream gradient
-  const float* kept;           // logits that the forward pass kept, or null
+  const char* kept;            // what the forward pass kept of the logits, or null
   float4* row_coef;            // [rpad]
   float* list_grad;            // [R, K]
   __nv_bfloat16* dl;           // [rpad, piece] gradient of one piece of the logits, or [piece, few rows]
@@ -68,7 +69,15 @@ struct HeadGradArgs {
   __nv_bfloat16* dw;           // [V, H] contiguous or null
 };
 
-int head_loss_kept(int R, int H, int V);                // row pitch of logits kept for the backward pass, or 0
+// What a forward pass keeps of the logits for a backward pass: of few rows the logits, [V, pitch] fp32; of many their
+// exponentials about the maxima of 128 columns, [rpad, pitch] fp16, and behind them those maxima (`part`).
+struct HeadKept {
+  long long bytes;             // 0: nothing is kept, the logits are computed again
+  int pitch;
+  long long part_at;           // many rows: where `part` begins
+  int tiles;                   // and its row length
+};
+HeadKept head_loss_kept(int R, int H, int V);
 int head_loss_vocab_tiles(int R, int V, bool kept);     // tiles of the statistics scratch
 int head_loss_grad_rows(int R);                         // rows (or row pitch) of the logits' gradient
 int head_loss_piece(int R, int V);                      // default backward piece

@@ -148,20 +148,21 @@ std::tuple<Tensor, Tensor, Tensor> head_loss_forward(Tensor h, Tensor weight, Te
   }
   osb::HeadStatsScratch p{};
   Tensor kept;
-  const int kept_pitch = keep ? osb::head_loss_kept(s.R, s.H, s.V) : 0;
-  if (kept_pitch > 0) {
-    kept = device_tensor({s.V, kept_pitch}, torch::kFloat32, h);
-    p.kept = kept.data_ptr<float>();
+  const osb::HeadKept keeps = keep ? osb::head_loss_kept(s.R, s.H, s.V) : osb::HeadKept{};
+  if (keeps.bytes > 0) {
+    kept = device_tensor({keeps.bytes}, torch::kUInt8, h);
+    p.kept = static_cast<char*>(kept.data_ptr());
   }
-  p.tiles = osb::head_loss_vocab_tiles(s.R, s.V, kept_pitch > 0);
+  p.tiles = osb::head_loss_vocab_tiles(s.R, s.V, keeps.bytes > 0);
   const long long parts = static_cast<long long>(s.rpad) * p.tiles;
   Carve size{nullptr};
-  size.take<float2>(parts);
+  size.take<float2>(keeps.part_at > 0 ? 0 : parts);
   size.take<float>(smoothing != 0.0 ? parts : 0);
   size.take<unsigned char>(R);
   const Scratch scratch(size.at);
   Carve c{scratch.base()};
-  p.part = c.take<float2>(parts);
+  p.part = c.take<float2>(keeps.part_at > 0 ? 0 : parts);
+  if (keeps.part_at > 0) p.part = reinterpret_cast<float2*>(p.kept + keeps.part_at);
   float* part_sum = c.take<float>(smoothing != 0.0 ? parts : 0);
   p.part_sum = smoothing != 0.0 ? part_sum : nullptr;
   t.active = c.take<unsigned char>(R);
@@ -190,7 +191,7 @@ std::tuple<OptTensor, OptTensor> head_loss_backward(Tensor saved, Tensor kept, T
   bind_state(s, static_cast<char*>(saved.data_ptr()));
   osb::HeadGradArgs a{};
   a.g = g.data_ptr<float>();
-  if (kept.defined()) a.kept = kept.data_ptr<float>();
+  if (kept.defined()) a.kept = static_cast<const char*>(kept.data_ptr());
   if (piece > 0) {
     TORCH_CHECK(piece % 256 == 0, "pieces are multiples of 256 columns");
     a.piece = static_cast<int>(std::min<int64_t>(piece, (V + 255) / 256 * 256));

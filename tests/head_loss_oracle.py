@@ -4,7 +4,9 @@ Bounds are elementwise.  ``logit``: an fp32 sum of H products is off by about sq
 steps of the sum of magnitudes; twice that is allowed.  A gradient adds half a step of
 bf16 (2^-8 relative) for the output and half a step for every term of the logits' gradient,
 which is rounded to bf16 once, besides what the logits' own error does to a probability
-(relative error of p: twice the logit's).
+(relative error of p: twice the logit's).  Steps of many rows keep their exponentials in fp16
+between the passes: half a step of fp16 (2^-11 relative, or 2^-40 of the largest of 128 columns,
+which is at most 1) on every probability.
 """
 
 import math
@@ -12,6 +14,7 @@ import math
 import torch
 
 BF16_HALF = 2.0 ** -8
+FP16_HALF = 2.0 ** -11
 FP32_HALF = 2.0 ** -24
 
 
@@ -58,7 +61,8 @@ def cross_entropy(h, weight, targets, g, ignore_index=-100, smoothing=0.0, z_los
     a = 1 + 2 * z_loss * lse
     dl = a[:, None] * p - smoothing / weight.shape[0]
     dl[at, t] -= 1 - smoothing
-    dl_err = (a[:, None] * p) * (2 * err + 2.0 ** -19)[:, None] + 4 * FP32_HALF * smoothing
+    dl_err = (a[:, None] * p) * (2 * err + 2.0 ** -19 + FP16_HALF)[:, None] + 4 * FP32_HALF * smoothing
+    dl_err = dl_err + a[:, None] * 2.0 ** -40 * p.amax(1, keepdim=True) if p.numel() else dl_err
     dl, dl_err = dl * gd[:, None], dl_err * gd.abs()[:, None]
     loss = torch.zeros(h.shape[0], dtype=torch.float64, device=h.device)
     loss_tol = torch.zeros_like(loss)
@@ -113,7 +117,8 @@ def topk_divergence(h, weight, ids, teacher, g, inv_temp=None, teacher_lse=None)
         loss_tol[r] = 2 * err + 16 * FP32_HALF * (size + 1)
         rows.append(r)
         dls.append(d * it * float(g[r]))
-        errs.append((q * (1 + ratio) * (4 * err + 2.0 ** -18) + p * 4 * FP32_HALF) * it * abs(float(g[r])))
+        off = (1 + ratio) * (q * (4 * err + 2.0 ** -18 + FP16_HALF) + 2.0 ** -40 * q.max())
+        errs.append((off + p * 4 * FP32_HALF) * it * abs(float(g[r])))
     if not rows:
         zero = torch.zeros(h.shape, dtype=torch.float64, device=h.device)
         return loss, loss_tol, zero, zero, torch.zeros_like(w), torch.zeros_like(w)
