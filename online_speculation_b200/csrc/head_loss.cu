@@ -1,4 +1,4 @@
-// Losses on a vocabulary head whose logits are not stored (or, for few rows, once): softmax cross entropy and the
+// Losses on a vocabulary head that never hold its logits in 32 bits but for few rows: softmax cross entropy and the
 // divergence from a teacher's listed logits, with the gradients of the hidden rows and of
 // the head.
 //
@@ -16,7 +16,8 @@
 //   own row over the tile's columns (running maximum, sum of exponentials) without shuffles,
 //   and lifts the listed logits out on the way.  Listed columns are left out of the sum: the
 //   mass of the rest comes out of a sum of its own, not of 1 - (something near 1).
-// * Backward goes over pieces of the vocabulary.  A piece's logits are recomputed, turned into
+// * Backward goes over pieces of the vocabulary.  A piece's logits, from what the forward pass kept of them (fp16
+//   exponentials, for few rows fp32 logits: head_loss_kept) or computed again, are turned into
 //   dl in bf16 (the type of the matrix instruction; 2^-9 rms against the same rounding of the
 //   outputs), and feed two products: dW of the piece is complete at once, dh adds up in fp32.
 //   Both read dl and their other operand in the layout they already have (MN-major
@@ -26,8 +27,6 @@
 //   lanes and rows in its columns.  A pass over few rows is the reading of the head, and a tile of
 //   256 lanes that holds 64 rows would spend four times the matrix instructions (and the clock that
 //   their power costs: 93 % tensor-pipe active at 1.5 GHz for 64 rows) on lanes that nobody looks at.
-//   Where those rows' logits are small next to the head, the forward pass leaves them for the backward pass,
-//   which then reads the head once instead of twice (head_loss_kept).
 // * Up to 128 rows keep dl as the sum of two bf16 numbers.  A row's gradient is mostly its target's
 //   entry: with few rows the rounding of single entries shows in the results (0.0027 relative where the
 //   rounding of the outputs alone is 0.0017), and the second half is nearly free, as the head is read
@@ -1564,15 +1563,6 @@ __global__ void __launch_bounds__(256) kept_scale_kernel(const HeadLossState s, 
   }
   const float4 coef = g.row_coef[m];
   const long long base = static_cast<long long>(s.row_of[m]) * s.K;
-  // listed columns of this block: from `from` on
-  int from = 0;
-  if (s.K > 1) {
-    int hi = s.K;
-    while (from < hi) {
-      const int mid = (from + hi) >> 1;
-      if (s.list_id[base + mid] < v0 + begin) from = mid + 1; else hi = mid;
-    }
-  }
 #pragma unroll
   for (int u = 0; u < kVecs; ++u) {
     const int v = begin + u * 2048 + threadIdx.x * 8;
@@ -1591,18 +1581,14 @@ __global__ void __launch_bounds__(256) kept_scale_kernel(const HeadLossState s, 
       for (int e = 0; e < 8; ++e)
         if (v + e >= cols) x[e] = 0.0f;
     }
-    for (; from < s.K; ++from) {
-      const int at = s.list_id[base + from] - v0 - (begin + u * 2048);
-      if (at >= 2048) break;
-      if (at / 8 == static_cast<int>(threadIdx.x) && at >= 0) {
-        const float value = g.list_grad[base + from];
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (e == at % 8) x[e] = value;
-      }
-    }
     if (v < end)
       *reinterpret_cast<uint4*>(dst + v) = make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7]));
+  }
+  // listed columns of this block, over what it wrote there
+  __syncthreads();
+  for (int i = threadIdx.x; i < s.K; i += 256) {
+    const int at = s.list_id[base + i] - v0;
+    if (at >= begin && at < min(cols, begin + kVecs * 2048)) dst[at] = __float2bfloat16_rn(g.list_grad[base + i]);
   }
 }
 
@@ -1767,12 +1753,15 @@ GemmArgs base_args(const HeadLossState& s) {
 
 }  // namespace
 
-// Row pitch of the logits that the forward pass keeps for a backward pass, 0 where that recomputes them.  A logit
-// kept is 8 bytes, written and read, and saves the second reading of the head with its products.  Forward and
-// hidden gradient, kept against recomputed: 192 rows of 3584 and 152064 columns 554 / 851 us, 16 rows of 3584
-// 426 / 582 us, 128 rows of 512 174 / 185 us, 256 rows of 64 218 / 215 us; 128 rows of 896 and 32768 columns
-// 75 / 80 us, 64 rows of 512 and 20000 columns 74 / 72 us (one more launch and allocation).  At most 256 MB, and at most
-// twice the head.
+// What a forward pass keeps for its backward pass.  Few rows: a logit kept is 8 bytes, written and read, and saves the
+// second reading of the head with its products.  Forward and hidden gradient, kept against computed again: 192 rows
+// of 3584 and 152064 columns 554 / 851 us, 16 rows of 3584 426 / 582 us, 128 rows of 512 174 / 185 us, 256 rows of
+// 64 218 / 215 us; 128 rows of 896 and 32768 columns 75 / 80 us, 64 rows of 512 and 20000 columns 74 / 72 us (one more
+// launch and allocation).  At most 256 MB, and at most twice the head.
+//
+// Many rows: 4 bytes a logit for 2 H operations.  Both gradients: 4096 rows of 3584 and 152064 columns 9.6 / 11.9 ms, 300
+// rows of 3584 1449 / 1832 us, 1024 rows of 512 and 50000 columns 214 / 228 us, 4096 rows of 256 and 152064
+// columns 1749 / 1695 us, 4096 rows of 64 and 32768 columns 385 / 335 us.  At most 2 GB.
 HeadKept head_loss_kept(int R, int H, int V) {
   HeadKept k{};
   if (few_rows(R)) {
@@ -1786,7 +1775,7 @@ HeadKept head_loss_kept(int R, int H, int V) {
   k.tiles = 2 * ceil_div(V, kBN);
   k.part_at = 2 * rpad * k.pitch;
   k.bytes = k.part_at + rpad * k.tiles * static_cast<long long>(sizeof(float2));
-  return k.part_at <= (2ll << 30) ? k : HeadKept{};
+  return H >= 384 && k.part_at <= (2ll << 30) ? k : HeadKept{};
 }
 
 // Partial statistics per row: one a warp of the launch, or two a tile of columns.

@@ -1,4 +1,4 @@
-"""Losses on a vocabulary head whose logits are not stored, and a teacher's top logits.
+"""Losses on a vocabulary head without a matrix of its logits, and a teacher's top logits.
 
 * :func:`head_cross_entropy`: softmax cross entropy of ``h @ weight.T``, with label
   smoothing and a penalty on the log-normaliser;
@@ -63,7 +63,7 @@ def _head_loss(h, weight, ids, teacher, teacher_lse, inv_temp, ignore_index, smo
 
 def head_cross_entropy(h: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *, ignore_index: int = -100,
                        label_smoothing: float = 0.0, z_loss: float = 0.0, piece: int | None = None) -> torch.Tensor:
-    """Cross entropy of ``softmax(h @ weight.T)`` per row (fp32 [R]), logits not stored.
+    """Cross entropy of ``softmax(h @ weight.T)`` per row (fp32 [R]).
 
     With l = h W^T, e = ``label_smoothing`` and z = ``z_loss``::
 
@@ -73,10 +73,13 @@ def head_cross_entropy(h: torch.Tensor, weight: torch.Tensor, targets: torch.Ten
     int64.  A row whose target is ``ignore_index`` gives 0 and takes no part in any product: its
     hidden row may hold anything.  A target outside the vocabulary raises on the CPU; on the GPU
     its row is ignored and ``workspace.check_status`` reports it.  Gradients are bf16, summed in
-    fp32.  ``piece`` (a multiple of 256): vocabulary columns the backward pass works on at a
-    time; its scratch is ``2 R piece`` bytes (256 MB without it).  Without it, a step of at most 256
-    (and H) rows on 32768 columns or more keeps its logits for the backward pass, ``4 R V`` bytes up to
-    256 MB, instead of computing them twice.
+    fp32.
+
+    Between the passes a step keeps 2 bytes a logit (``2 R V``, up to 2 GB; H at least 384) or, of at most
+    256 (and H) rows on 32768 columns or more, 4 bytes (up to 256 MB); larger ones, and all others,
+    keep nothing and compute the logits twice.  ``piece`` (a multiple of 256) bounds the memory: nothing is
+    kept, and the backward pass works on that many vocabulary columns at a time with ``2 R piece`` bytes
+    of scratch (twice that up to 128 rows; 256 MB without it).
 
     A training step that is captured into a CUDA graph takes its gradients with
     ``torch.autograd.grad``; no eager graph of the same leaves may be alive meanwhile.
@@ -98,7 +101,7 @@ def head_cross_entropy(h: torch.Tensor, weight: torch.Tensor, targets: torch.Ten
 def head_topk_divergence(h: torch.Tensor, weight: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor, *,
                          inv_temp: torch.Tensor | None = None, teacher_lse: torch.Tensor | None = None,
                          piece: int | None = None) -> torch.Tensor:
-    """KL(teacher || softmax(inv_temp * h @ weight.T)) per row (fp32 [R]), logits not stored.
+    """KL(teacher || softmax(inv_temp * h @ weight.T)) per row (fp32 [R]).
 
     ``ids`` [R, K] (int32 or int64) and ``teacher`` [R, K] (fp32 or bf16 logits) list the teacher's
     best columns of every row, in any order, K at most 512; a slot with a negative id or a logit

@@ -370,6 +370,42 @@ def test_kept_logits(cuda, rows, hidden, vocab, listed):
         oracle.within(only, want[2], want[3], "dh alone")
 
 
+def test_kept_exponentials_in_pieces(cuda):
+    """Many rows, several pieces whose length is no multiple of a block's columns, targets around the seams."""
+    rows, hidden, vocab = 2560, 392, 60000
+    h, w, t, gen = oracle.make_inputs(rows, hidden, vocab, 17, cuda)
+    t[::2] = torch.randint(52100, 57400, (rows // 2,), generator=gen).to(cuda)
+    t[5::40] = -100
+    g = torch.randn(rows, generator=gen).to(cuda)
+    want = oracle.cross_entropy(h, w, t, g, smoothing=0.1)
+    h.requires_grad_()
+    w.requires_grad_()
+    loss = K.head_cross_entropy(h, w, t, label_smoothing=0.1)
+    for got, i in zip((loss.detach(), *_grads(loss, h, w, g)), (0, 2, 4)):
+        oracle.within(got, want[i], want[i + 1], i)
+
+
+@pytest.mark.parametrize("k", [1, 100])
+def test_kept_exponentials_of_lists(cuda, k):
+    """Rows sure of one unlisted column, listed columns at the ends, a list in one block of columns."""
+    rows, hidden, vocab = 300, 400, 20001
+    h, w, t, gen = oracle.make_inputs(rows, hidden, vocab, 18, cuda)
+    h = (h + 12 * w[t] * (torch.arange(rows, device=cuda) % 3 == 0)[:, None]).bfloat16()
+    ids = torch.randint(0, vocab, (rows, k), generator=gen).to(cuda)
+    ids[::4] = 9000 + torch.arange(k, device=cuda)
+    ids[1, 0], ids[2, 0] = 0, vocab - 1
+    ids[7] = -1
+    teacher = torch.randn(rows, k, generator=gen).to(cuda)
+    lse = teacher.logsumexp(1) + math.log(3.0)
+    g = torch.randn(rows, generator=gen).to(cuda)
+    want = oracle.topk_divergence(h, w, ids, teacher, g, None, lse)
+    h.requires_grad_()
+    w.requires_grad_()
+    loss = K.head_topk_divergence(h, w, ids, teacher, teacher_lse=lse)
+    for got, i in zip((loss.detach(), *_grads(loss, h, w, g)), (0, 2, 4)):
+        oracle.within(got, want[i], want[i + 1], i)
+
+
 def test_what_is_kept(cuda):
     """A step keeps the logits of few rows until its graph goes; without gradients, or with a piece, nothing."""
     rows, hidden, vocab = 16, 1024, 65792
