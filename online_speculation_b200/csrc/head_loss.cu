@@ -84,6 +84,7 @@ struct GemmArgs {
   int H, V;
   int v0, cols;            // this piece: first vocabulary row, columns that exist
   int bn;                  // rows in columns: how many columns, a multiple of 16
+  int chains, chain;       // rows in columns: sums of that many blocks of the reduction each, side by side in the accumulator
   int tiles_n;             // column tiles of the accumulator grid
   int lo;                  // rows in columns: where a row of the logits' gradient holds what rounding to bf16 took
                            // from its first half (0: not kept)
@@ -570,6 +571,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW
         const bool mn_a = MODE == kProd && (it.kind == (FEW ? 0 : 1)), mn_b = MODE == kProd;
         const int columns = FEW && it.kind == 0 ? (MODE == kProd && a.lo > 0 ? 2 * a.bn : a.bn) : kBN;
         const uint32_t idesc = idesc_bf16_f32(kBM, columns) | (mn_a ? 1u << 15 : 0u) | (mn_b ? 1u << 16 : 0u);
+        constexpr bool kChains = FEW && MODE != kProd;
+        uint32_t dk = d;
+        int from = it.kb0, turn = a.chain;
         for (int kb = it.kb0; kb < it.kb1; ++kb) {
           if (!mbar_wait(&full[stage], phase, a.status, kErrMmaWait)) {
             ok = false;
@@ -577,11 +581,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW
           }
           tc_fence_after();
           const uint32_t pa = base + stage * stage_bytes, pb = pa + sb.a;
+          if (kChains && kb == turn) {
+            dk += a.bn;
+            from = kb;
+            turn += a.chain;
+          }
 #pragma unroll
           for (int k = 0; k < kBK / 16; ++k) {
             const uint64_t ad = mn_a ? sdesc_mn_sw128(pa + k * 2048, kBox, 1024) : sdesc_k_sw128(pa + k * 32);
             const uint64_t bd = mn_b ? sdesc_mn_sw128(pb + k * 2048, kBox, 1024) : sdesc_k_sw128(pb + k * 32);
-            pair_mma(d, ad, bd, idesc, (kb > it.kb0 || k > 0) ? 1u : 0u);
+            pair_mma(dk, ad, bd, idesc, (kb > from || k > 0) ? 1u : 0u);
           }
           pair_commit(&empty[stage]);
           if (++stage == stages) {
@@ -759,6 +768,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW
           const int t0 = c * 32, t = t0 + lane;
           float x[32];
           tmem_ld32(t_acc + t0, x);
+          for (int n = 1; n < a.chains; ++n) {
+            float y[32];
+            tmem_ld32(t_acc + n * a.bn + t0, y);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) x[j] += y[j];
+          }
           if (MODE == kStats) {
             if (a.kept) {
               // lanes outside the vocabulary are cut off by the map: a warp's columns are its own (see lane_slot)
@@ -1375,8 +1390,9 @@ __global__ void __launch_bounds__(128) gather_rows_kernel(const HeadLossState s)
 // in fp64 from fp32 sums: a divergence is a small difference of logarithms.
 //
 // The tensor core's sums of H products come out a little short (its additions truncate: about 2e-6 of a
-// logit at H = 3584).  Listed logits and normaliser share that, so most of it cancels in a loss; listed
-// logits summed again in fp32 made the losses worse (1.2e-6 for 0.9e-6 relative, 64 rows of 152064).
+// logit at H = 3584 in one chain).  Listed logits and normaliser share that, so most of it cancels in a loss; listed
+// logits summed again in fp32 made the losses worse (1.2e-6 for 0.9e-6 relative, 64 rows of 152064).  Up to 128
+// rows have room for several chains (2.0e-7, at no time).
 __global__ void __launch_bounds__(128) finish_rows_kernel(const HeadLossState s, const HeadStatsScratch p) {
   __shared__ double buf_d[4];
   __shared__ float buf_f[4];
@@ -1746,6 +1762,10 @@ GemmArgs base_args(const HeadLossState& s) {
   a.rpad = s.rpad;
   a.slot = kHalf;
   a.bn = few_rows(s.R) ? ceil_div(s.R, 16) * 16 : kBN;
+  // the tensor core truncates at every addition: shorter chains, added in fp32, are off by less.  Blocks in turn took 251
+  // us where chains of neighbours take 226 (64 rows of 3584 on 152064 columns).
+  a.chain = ceil_div(ceil_div(s.H, kBK), std::max(1, std::min(4, kBN / a.bn)));
+  a.chains = ceil_div(ceil_div(s.H, kBK), a.chain);
   a.lo = s.R <= kSplitRows ? ceil_div(s.R, 64) * 64 : 0;
   a.status = s.status;
   return a;

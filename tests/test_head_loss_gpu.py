@@ -66,13 +66,14 @@ def test_ignored_rows_may_hold_anything(cuda, pattern):
     assert bool((dh[drop] == 0).all()) and bool((loss[drop] == 0).all())
 
 
+@pytest.mark.parametrize("rows,hidden,vocab,piece", [(90, 256, 1500, 512), (290, 400, 1500, None), (90, 256, 33000, None)])
 @pytest.mark.parametrize("need", ["h", "w"])
-def test_one_gradient(cuda, need):
-    h, w, t, gen = oracle.make_inputs(90, 256, 1500, 9, cuda)
-    g = torch.randn(90, generator=gen).to(cuda)
+def test_one_gradient(cuda, need, rows, hidden, vocab, piece):
+    h, w, t, gen = oracle.make_inputs(rows, hidden, vocab, 9, cuda)
+    g = torch.randn(rows, generator=gen).to(cuda)
     want = oracle.cross_entropy(h, w, t, g)
     leaf = (h if need == "h" else w).requires_grad_()
-    loss = K.head_cross_entropy(h, w, t, piece=512)
+    loss = K.head_cross_entropy(h, w, t, piece=piece)
     (got,) = torch.autograd.grad(loss, [leaf], g)
     i = 2 if need == "h" else 4
     oracle.within(got, want[i], want[i + 1], need)
@@ -402,8 +403,11 @@ def test_kept_exponentials_of_lists(cuda, k):
     h.requires_grad_()
     w.requires_grad_()
     loss = K.head_topk_divergence(h, w, ids, teacher, teacher_lse=lse)
-    for got, i in zip((loss.detach(), *_grads(loss, h, w, g)), (0, 2, 4)):
+    first = torch.autograd.grad(loss, [h, w], g, retain_graph=True)
+    again = torch.autograd.grad(loss, [h, w], g)
+    for got, i in zip((loss.detach(), *first), (0, 2, 4)):
         oracle.within(got, want[i], want[i + 1], i)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
 
 
 def test_what_is_kept(cuda):
