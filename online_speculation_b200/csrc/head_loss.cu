@@ -737,6 +737,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW
         tc_fence_after();
       }
       const uint32_t t_acc = tmem + lane_base + acc * kBN;
+      bool released = false;
+      auto release = [&]() {                                // the accumulator has been read
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) remote_arrive(map_shared_rank(smem_u32(&tempty[acc]), 0));
+        released = true;
+      };
 
       if (FEW && MODE != kProd) {
         // lanes are vocabulary columns, this thread's is `col`; chunks of 32 rows
@@ -889,9 +896,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW
         if (m0 < rows) {
           float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
+          for (int c = 0; c < kBN / 64; ++c) tmem_ld32(t_acc + set * (kBN / 2) + c * 32, x[c]);
+          release();
+#pragma unroll
           for (int c = 0; c < kBN / 64; ++c) {
             const int col = first + c * 32;
-            tmem_ld32(t_acc + set * (kBN / 2) + c * 32, x[c]);
             if (col + 32 > a.V) {
 #pragma unroll
               for (int j = 0; j < 32; ++j) {
@@ -1135,9 +1144,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW
       }
       if (!FEW && MODE != kProd && more) fetch_id();
       if (!empty_sum) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) remote_arrive(map_shared_rank(smem_u32(&tempty[acc]), 0));
+        if (!released) release();
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1;
       }
