@@ -1638,6 +1638,8 @@ __global__ void __launch_bounds__(128) kept_listed_kernel(const HeadLossState s,
 // Sums the parts of the hidden gradient.  `mend`: dl had its listed entries, which are most of a row's gradient, in
 // one bf16 number; what rounding took from them times their head rows comes on top here.  (Relative error
 // of dh for a loss with one target 0.0024 without, 0.0017 with it: that of rounding dh itself.)
+constexpr int kMendAhead = 16;   // 192 rows of 3584, lists of 64: 40 us; 8 left to the compiler 64 us
+
 __global__ void __launch_bounds__(128) hidden_grad_kernel(const HeadLossState s, const HeadGradArgs g, int mend) {
   __shared__ float lost[kHeadMaxListed];
   __shared__ int column[kHeadMaxListed];
@@ -1662,14 +1664,21 @@ __global__ void __launch_bounds__(128) hidden_grad_kernel(const HeadLossState s,
   uint4 v = make_uint4(0, 0, 0, 0);
   if (m >= 0) {
     float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 8
-    for (int k = 0; k < listed; ++k) {
-      const uint4 w = __ldg(reinterpret_cast<const uint4*>(s.w + static_cast<long long>(column[k]) * s.ldw) + i);
-      const unsigned u[4] = {w.x, w.y, w.z, w.w};
+    for (int k0 = 0; k0 < listed; k0 += kMendAhead) {
+      uint4 w[kMendAhead];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[2 * e] = fmaf(lost[k], __uint_as_float(u[e] << 16), x[2 * e]);
-        x[2 * e + 1] = fmaf(lost[k], __uint_as_float(u[e] & 0xFFFF0000u), x[2 * e + 1]);
+      for (int a = 0; a < kMendAhead; ++a)
+        if (k0 + a < listed)
+          w[a] = __ldg(reinterpret_cast<const uint4*>(s.w + static_cast<long long>(column[k0 + a]) * s.ldw) + i);
+#pragma unroll
+      for (int a = 0; a < kMendAhead; ++a) {
+        if (k0 + a >= listed) break;
+        const unsigned u[4] = {w[a].x, w[a].y, w[a].z, w[a].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[2 * e] = fmaf(lost[k0 + a], __uint_as_float(u[e] << 16), x[2 * e]);
+          x[2 * e + 1] = fmaf(lost[k0 + a], __uint_as_float(u[e] & 0xFFFF0000u), x[2 * e + 1]);
+        }
       }
     }
 #pragma unroll 4
@@ -1841,8 +1850,9 @@ int head_loss_splits(int R, int H, int piece, int V, bool with_dw) {
     if (want > 1 && tiles >= 2 * pairs) break;          // enough tiles as they are
     const int per = ceil_div(kb, want), splits = ceil_div(kb, per), weigh = few ? per + per / 2 : per;
     if (with_dw && weigh <= (tiles * weigh * splits + other) / pairs) return splits;
-    // a tile's end and its partial sums weigh about four blocks
-    const long long c = static_cast<long long>(ceil_div(tiles * splits, pairs)) * (per + 4);
+    // a tile's end weighs about four blocks, and a partial sum's way through memory a block per MB (few rows, whose blocks
+    // wait for the head, per 3 MB): nearly equal rounds would otherwise take 21 parts for 5 of 192 x 3584
+    const long long c = static_cast<long long>(ceil_div(tiles * splits, pairs)) * (per + 4) + splits * bytes / ((few ? 3ll : 1ll) << 20);
     if (c < cost) {
       cost = c;
       best = splits;
