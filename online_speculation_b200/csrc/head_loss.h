@@ -31,7 +31,9 @@ struct HeadLossState {
   float* list_mass;            // [R, K] teacher mass (divergence), unused for cross entropy
   float* list_logit;           // [R, K] student logits of the listed columns
   float* rest_mass;            // [R] teacher mass outside the list (divergence)
-  float4* row_stat;            // [R]: lse, mass of the unlisted columns, factor of p on unlisted columns, unused
+  float* all_mass;             // [R] listed and rest mass (divergence): 1 but for a teacher whose list was rounded
+  float4* row_stat;            // [R]: lse, mass of the unlisted columns, factor of p on unlisted columns, factor on
+                               // listed ones (divergence)
   float* loss;                 // [R]
   int* status;
 };

@@ -71,6 +71,7 @@ size_t bind_state(osb::HeadLossState& s, char* base) {
   s.list_logit = c.take<float>(listed);
   s.list_mass = c.take<float>(s.divergence ? listed : 0);
   s.rest_mass = c.take<float>(s.divergence ? s.R : 0);
+  s.all_mass = c.take<float>(s.divergence ? s.R : 0);
   s.row_stat = c.take<float4>(s.R);
   return c.at;
 }

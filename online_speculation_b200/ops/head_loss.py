@@ -111,7 +111,9 @@ def head_topk_divergence(h: torch.Tensor, weight: torch.Tensor, ids: torch.Tenso
     Without ``teacher_lse`` the teacher is the softmax of its listed logits.  With it (fp32 [R], the
     logsumexp of all of the teacher's scaled logits, as :func:`top_logits` returns it) the listed
     columns keep their true masses and all others together are one more outcome on both sides
-    (where the list holds every column there is none).
+    (where the list holds every column there is none).  Masses are taken as they are: those of a teacher
+    whose logits were rounded sum to a little more or less than 1, and the gradient is that of the loss
+    with them.
 
     A row without a listed column gives 0 and takes no part in any product.  A column beyond the
     vocabulary raises on the CPU; on the GPU its slot is empty and ``workspace.check_status``
