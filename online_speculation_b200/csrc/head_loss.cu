@@ -113,6 +113,18 @@ struct GemmArgs {
 // halves, all rows of one of them.
 __host__ __device__ inline int row_boxes(const GemmArgs& a) { return ((a.lo > 0 ? a.bn : a.bn / 2) + 63) / 64; }
 
+// Rows in columns: columns of the accumulator, and the most chains of a sum that stand in it side by side.
+__host__ __device__ constexpr int row_columns(int R) { return (R + 15) / 16 * 16; }
+__host__ __device__ constexpr int most_chains(int bn) { return kBN / bn < 4 ? kBN / bn : 4; }
+
+// The epilogue loads 32 columns at a time, up to the last row's, of every chain.
+constexpr bool loads_stay_inside() {
+  for (int R = 1; R <= kFewRows; ++R)
+    if ((most_chains(row_columns(R)) - 1) * row_columns(R) + (R + 31) / 32 * 32 > kBN) return false;
+  return true;
+}
+static_assert(loads_stay_inside(), "the last chain's loads end inside the accumulator");
+
 struct StageBytes {
   int a, b;
 };
@@ -774,12 +786,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW
         for (int c = 0; c < chunks && first < stop; ++c) {
           const int t0 = c * 32, t = t0 + lane;
           float x[32];
-          tmem_ld32(t_acc + t0, x);
-          for (int n = 1; n < a.chains; ++n) {
-            float y[32];
-            tmem_ld32(t_acc + n * a.bn + t0, y);
+          if (t0 < rows) {
+            tmem_ld32(t_acc + t0, x);
+            for (int n = 1; n < a.chains; ++n) {
+              float y[32];
+              tmem_ld32(t_acc + n * a.bn + t0, y);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) x[j] += y[j];
+              for (int j = 0; j < 32; ++j) x[j] += y[j];
+            }
+          } else {
+            // the half of the last box behind the rows: the last chain's columns would end behind the accumulator
+#pragma unroll
+            for (int j = 0; j < 32; ++j) x[j] = 0.0f;
           }
           if (MODE == kStats) {
             if (a.kept) {
@@ -1781,10 +1799,10 @@ GemmArgs base_args(const HeadLossState& s) {
   a.list_id = s.list_id;
   a.rpad = s.rpad;
   a.slot = kHalf;
-  a.bn = few_rows(s.R) ? ceil_div(s.R, 16) * 16 : kBN;
+  a.bn = few_rows(s.R) ? row_columns(s.R) : kBN;
   // the tensor core truncates at every addition: shorter chains, added in fp32, are off by less.  Blocks in turn took 251
   // us where chains of neighbours take 226 (64 rows of 3584 on 152064 columns).
-  a.chain = ceil_div(ceil_div(s.H, kBK), std::max(1, std::min(4, kBN / a.bn)));
+  a.chain = ceil_div(ceil_div(s.H, kBK), most_chains(a.bn));
   a.chains = ceil_div(ceil_div(s.H, kBK), a.chain);
   a.lo = s.R <= kSplitRows ? ceil_div(s.R, 64) * 64 : 0;
   a.status = s.status;

@@ -1,0 +1,35 @@
+"""Edges of the vocabulary-head losses and top logits on the kernels."""
+
+import pytest
+import torch
+
+import head_loss_oracle as oracle
+from online_speculation_b200.ops import kernels as K
+from online_speculation_b200.ops import workspace
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("rows", [65, 72, 80])
+@pytest.mark.parametrize("listed", [0, 5])
+def test_two_tiles_a_pair_of_65_to_80_rows(cuda, rows, listed):
+    """Logits computed again with rows in columns, in three chains of 80 columns, both accumulators used."""
+    hidden, vocab = 512, 24000
+    h, w, t, gen = oracle.make_inputs(rows, hidden, vocab, rows, cuda)
+    g = torch.randn(rows, generator=gen).to(cuda)
+    if listed:
+        ids = torch.randint(0, vocab, (rows, listed), generator=gen).to(cuda)
+        teacher = torch.randn(rows, listed, generator=gen).to(cuda)
+        lse = teacher.logsumexp(1) + 0.5
+        want = oracle.topk_divergence(h, w, ids, teacher, g, None, lse)
+    else:
+        want = oracle.cross_entropy(h, w, t, g, smoothing=0.1)
+    h.requires_grad_()
+    w.requires_grad_()
+    if listed:
+        loss = K.head_topk_divergence(h, w, ids, teacher, teacher_lse=lse)
+    else:
+        loss = K.head_cross_entropy(h, w, t, label_smoothing=0.1)
+    for got, i in zip((loss.detach(), *torch.autograd.grad(loss, [h, w], g)), (0, 2, 4)):
+        oracle.within(got, want[i], want[i + 1], i)
+    workspace.check_status(cuda)
