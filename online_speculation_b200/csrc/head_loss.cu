@@ -668,7 +668,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW
     auto fetch_row = [&](const Item& n) {
       const int m = n.m0 + rank * kHalf + quarter * 32 + lane;
       next_row = m < rows ? a.row_of[m] : -1;
-      if (MODE == kGrad && m < rows) next_coef = a.row_coef[m];
+      // zero behind the last row, up to its tile's end: another row's normaliser could overflow there, and the head
+      // gradient's product reads those rows
+      if (MODE == kGrad) next_coef = a.row_coef[m];
     };
     float next_scale = kLog2e;
     auto fetch_id = [&]() {

@@ -33,3 +33,18 @@ def test_two_tiles_a_pair_of_65_to_80_rows(cuda, rows, listed):
     for got, i in zip((loss.detach(), *torch.autograd.grad(loss, [h, w], g)), (0, 2, 4)):
         oracle.within(got, want[i], want[i + 1], i)
     workspace.check_status(cuda)
+
+
+def test_low_logits_of_many_rows(cuda):
+    """Every logit near -120, so that exponentials about another row's normaliser, or about none, overflow: what stands
+    behind the last row must not reach dW.  Several row tiles, two items a CTA pair, logits computed again."""
+    rows, hidden, vocab = 701, 64, 10000
+    h, w, t, gen = oracle.make_inputs(rows, hidden, vocab, 3, cuda)
+    h[:, 0], w[:, 0] = -120.0, 1.0
+    g = torch.randn(rows, generator=gen).to(cuda)
+    want = oracle.cross_entropy(h, w, t, g)
+    h.requires_grad_()
+    w.requires_grad_()
+    loss = K.head_cross_entropy(h, w, t)
+    for got, i in zip((loss.detach(), *torch.autograd.grad(loss, [h, w], g)), (0, 2, 4)):
+        oracle.within(got, want[i], want[i + 1], i)
