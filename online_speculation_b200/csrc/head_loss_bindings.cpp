@@ -234,7 +234,9 @@ struct HeadLossNode : public torch::autograd::Function<HeadLossNode> {
                         const Tensor& status) {
     auto [loss, saved, kept] = head_loss_forward(h, weight, ids, teacher, teacher_lse, inv_temp, ignore_index, smoothing,
                                            z_loss, keep, status);
-    ctx->save_for_backward({saved, weight, given(inv_temp) ? *inv_temp : Tensor(), status, kept});
+    ctx->save_for_backward({saved, weight, given(inv_temp) ? *inv_temp : Tensor(), kept});
+    // one word a device, shared by all kernels and reset when an error is reported: no input whose changes count
+    ctx->saved_data["status"] = status;
     ctx->saved_data["k"] = given(teacher) ? ids.size(1) : 1;
     ctx->saved_data["divergence"] = given(teacher);
     ctx->saved_data["rest"] = given(teacher_lse);
@@ -252,9 +254,9 @@ struct HeadLossNode : public torch::autograd::Function<HeadLossNode> {
     OptTensor inv_temp;
     if (saved[2].defined()) inv_temp = saved[2];
     auto& d = ctx->saved_data;
-    auto [dh, dw] = head_loss_backward(saved[0], saved[4], saved[1], inv_temp, g, d["k"].toInt(), d["divergence"].toBool(),
+    auto [dh, dw] = head_loss_backward(saved[0], saved[3], saved[1], inv_temp, g, d["k"].toInt(), d["divergence"].toBool(),
                                        d["rest"].toBool(), d["smoothing"].toDouble(), d["z"].toDouble(),
-                                       ctx->needs_input_grad(0), ctx->needs_input_grad(1), d["piece"].toInt(), saved[3]);
+                                       ctx->needs_input_grad(0), ctx->needs_input_grad(1), d["piece"].toInt(), d["status"].toTensor());
     torch::autograd::variable_list out(12);
     if (given(dh)) out[0] = *dh;
     if (given(dw)) out[1] = *dw;

@@ -48,3 +48,39 @@ def test_low_logits_of_many_rows(cuda):
     loss = K.head_cross_entropy(h, w, t)
     for got, i in zip((loss.detach(), *torch.autograd.grad(loss, [h, w], g)), (0, 2, 4)):
         oracle.within(got, want[i], want[i + 1], i)
+
+
+def test_training_after_rollouts_in_inference_mode(cuda, monkeypatch):
+    """The package's first kernel may run in inference mode: what it makes for the device serves training too."""
+    monkeypatch.setattr(workspace, "_buffers", {})
+    h, w, t, gen = oracle.make_inputs(20, 64, 300, 4, cuda)
+    with torch.inference_mode():
+        K.head_cross_entropy(h, w, t)
+    g = torch.randn(20, generator=gen).to(cuda)
+    want = oracle.cross_entropy(h, w, t, g)
+    h.requires_grad_()
+    w.requires_grad_()
+    loss = K.head_cross_entropy(h, w, t)
+    dh, dw = torch.autograd.grad(loss, [h, w], g)
+    oracle.within(dh, want[2], want[3], "dh")
+    oracle.within(dw, want[4], want[5], "dW")
+
+
+def test_error_reported_between_the_passes(cuda):
+    """A bad target is reported and its row left out; the step it was in, and others, still have their gradients."""
+    h, w, t, gen = oracle.make_inputs(20, 64, 300, 4, cuda)
+    bad = t.clone()
+    bad[3] = 300
+    g = torch.randn(20, generator=gen).to(cuda)
+    without = torch.where(bad == 300, -100, t)
+    want = oracle.cross_entropy(h, w, without, g)
+    h.requires_grad_()
+    w.requires_grad_()
+    loss, other = K.head_cross_entropy(h, w, bad), K.head_cross_entropy(h, w, without)
+    with pytest.raises(RuntimeError, match="out of range"):
+        workspace.check_status(cuda)
+    for x in (loss, other):
+        dh, dw = torch.autograd.grad(x, [h, w], g)
+        oracle.within(dh, want[2], want[3], "dh")
+        oracle.within(dw, want[4], want[5], "dW")
+    workspace.check_status(cuda)
