@@ -6,6 +6,9 @@
   at zero when it finishes,
 * ``status``: one int32 word that bounded device-side waits write an error code
   into instead of hanging.  :func:`check_status` turns it into an exception.
+
+Buffers live as long as the process, so they are ordinary tensors also when the first call that needs
+one runs in inference mode: an inference tensor could not be reset outside of it.
 """
 
 from __future__ import annotations
@@ -39,7 +42,8 @@ def _get(device: torch.device, name: str, factory) -> torch.Tensor:
         with _lock:
             buffer = _buffers.get(key)
             if buffer is None:
-                buffer = factory(torch.device("cuda", index))
+                with torch.inference_mode(False):
+                    buffer = factory(torch.device("cuda", index))
                 _buffers[key] = buffer
     return buffer
 
@@ -85,7 +89,8 @@ def scratch(device: torch.device, name: str, numel: int, dtype: torch.dtype) -> 
     with _lock:
         buffer = _buffers.get(key)
         if buffer is None or buffer.numel() < numel or buffer.dtype != dtype:
-            buffer = torch.empty(numel, dtype=dtype, device=torch.device("cuda", index))
+            with torch.inference_mode(False):
+                buffer = torch.empty(numel, dtype=dtype, device=torch.device("cuda", index))
             _buffers[key] = buffer
     return buffer[:numel]
 

@@ -84,3 +84,21 @@ def test_error_reported_between_the_passes(cuda):
         oracle.within(dh, want[2], want[3], "dh")
         oracle.within(dw, want[4], want[5], "dW")
     workspace.check_status(cuda)
+
+
+def test_error_after_a_first_use_in_inference_mode(cuda, monkeypatch):
+    monkeypatch.setattr(workspace, "_buffers", {})
+    h, w, t, _ = oracle.make_inputs(20, 64, 300, 4, cuda)
+    t[3] = 300
+    with torch.inference_mode():
+        K.head_cross_entropy(h, w, t)
+    with pytest.raises(RuntimeError, match="out of range"):
+        workspace.check_status(cuda)
+    workspace.check_status(cuda)
+
+
+def test_scratch_first_made_in_inference_mode(cuda, monkeypatch):
+    monkeypatch.setattr(workspace, "_buffers", {})
+    with torch.inference_mode():
+        buffer = workspace.scratch(cuda, "test", 8, torch.float32)
+    assert not buffer.is_inference() and not workspace.scratch(cuda, "test", 4, torch.float32).is_inference()
