@@ -3,7 +3,8 @@
 // the head.
 //
 //   l = h W^T,  q = softmax(it * l)                       h [R, H], W [V, H], bf16
-//   dl[r, v] = A_r q[r, v] - C_r on the unlisted columns, a stored value on the listed ones
+//   dl[r, v] = A_r q[r, v] - C_r on the unlisted columns (q for a divergence: softmax over those alone), a stored
+//   value on the listed ones
 //   dh = dl W,  dW = dl^T h
 //
 // A row's listed columns are its target, or the teacher's columns; everything dense about
@@ -373,13 +374,14 @@ __device__ __forceinline__ void seek_rows(const int* list_id, int K, const int* 
     if (t0 + j * 128 < rows) cursors[t0 + j * 128] = make_int2(lo[j], lo[j] < K ? id[j] : INT_MAX);
 }
 
-// A row's coefficients of the logits' gradient: {it log2 e, lse log2 e, A, C} of A exp(it l - lse) - C.
+// A row's coefficients of the logits' gradient: {it log2 e, lse log2 e, A, C} of A exp(it l - lse) - C.  A divergence's are
+// about the normaliser of the unlisted columns, that of a cross entropy about all.
 __device__ __forceinline__ float4 row_coefficients(const HeadLossState& s, const float* g, int r) {
   const float4 st = s.row_stat[r];
   const float it = s.inv_temp != nullptr ? s.inv_temp[r] : 1.0f;
   const float up = g[r] * it;
   const float flat = s.divergence ? 0.0f : s.smoothing / static_cast<float>(s.V);
-  return make_float4(it * kLog2e, st.x * kLog2e, up * st.z, up * flat);
+  return make_float4(it * kLog2e, (s.divergence ? st.y : st.x) * kLog2e, up * st.z, up * flat);
 }
 
 // The gradient of the listed logit `at` of row r.  Written so that every kernel gets the same bits: the rest that
@@ -1464,7 +1466,7 @@ __global__ void __launch_bounds__(128) finish_rows_kernel(const HeadLossState s,
       mx != -INFINITY ? part_rest * exp((static_cast<double>(mx) - static_cast<double>(top)) * it) : part_rest;
   const double lse = static_cast<double>(top) * it + log(rest + listed);
   const double q_rest = rest / (rest + listed);
-  double loss, factor, listed_factor = 0.0;
+  double loss, factor, second = q_rest, listed_factor = 0.0;
   if (!s.divergence) {
     const double target = s.list_logit[base];
     const double hot = listed > 0.0 ? log1p(rest / listed) : lse - target;
@@ -1483,16 +1485,20 @@ __global__ void __launch_bounds__(128) finish_rows_kernel(const HeadLossState s,
     loss = block_combine(sum, buf_d, add);
     // Every log q of the loss brings its mass times q_v to the gradient: all masses, whose sum is above one where a
     // teacher's logits were rounded and its normaliser was not (bf16 logits near 20: up to 6 %).
-    factor = listed_factor = s.all_mass[r];
+    //
+    // On the unlisted columns q_v = q_rest r_v, with r their own softmax, and the rest takes rest_mass r_v off.  r is
+    // at most one however little mass the student leaves there; q_v and rest_mass / q_rest leave fp32 where listed logits
+    // lead by 88, and rest leaves fp64 where they lead by 745.
+    listed_factor = s.all_mass[r];
+    const double lse_rest = part_rest == 0.0 ? -INFINITY : static_cast<double>(mx) * it + log(part_rest);
     const double rest_mass = s.rest_bucket ? static_cast<double>(s.rest_mass[r]) : 0.0;
-    if (rest_mass != 0.0 && rest > 0.0) {
-      loss += rest_mass * log(rest_mass / q_rest);
-      factor -= rest_mass / q_rest;
-    }
+    if (rest_mass != 0.0) loss += rest_mass * (log(rest_mass) - (lse_rest - lse));
+    factor = listed_factor * q_rest - rest_mass;
+    second = part_rest == 0.0 ? lse : lse_rest;   // no unlisted column
   }
   if (tid == 0) {
     s.loss[r] = static_cast<float>(loss);
-    s.row_stat[r] = make_float4(static_cast<float>(lse), static_cast<float>(q_rest), static_cast<float>(factor),
+    s.row_stat[r] = make_float4(static_cast<float>(lse), static_cast<float>(second), static_cast<float>(factor),
                                 static_cast<float>(listed_factor));
   }
 }

@@ -32,8 +32,8 @@ struct HeadLossState {
   float* list_logit;           // [R, K] student logits of the listed columns
   float* rest_mass;            // [R] teacher mass outside the list (divergence)
   float* all_mass;             // [R] listed and rest mass (divergence): 1 but for a teacher whose list was rounded
-  float4* row_stat;            // [R]: lse, mass of the unlisted columns, factor of p on unlisted columns, factor on
-                               // listed ones (divergence)
+  float4* row_stat;            // [R]: lse; then cross entropy: mass of the unlisted columns, factor of q, unused; divergence:
+                               // lse of the unlisted columns, factor of their own softmax, factor of q on listed ones
   float* loss;                 // [R]
   int* status;
 };

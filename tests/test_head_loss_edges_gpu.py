@@ -3,6 +3,7 @@
 import pytest
 import torch
 
+import head_loss_masses as masses
 import head_loss_oracle as oracle
 from online_speculation_b200.ops import kernels as K
 from online_speculation_b200.ops import workspace
@@ -102,3 +103,25 @@ def test_scratch_first_made_in_inference_mode(cuda, monkeypatch):
     with torch.inference_mode():
         buffer = workspace.scratch(cuda, "test", 8, torch.float32)
     assert not buffer.is_inference() and not workspace.scratch(cuda, "test", 4, torch.float32).is_inference()
+
+
+@pytest.mark.parametrize("rows,hidden,vocab", [(20, 512, 33000), (100, 512, 3000), (200, 512, 33000), (200, 512, 3000),
+                                               (300, 512, 3000), (300, 256, 3000)])
+@pytest.mark.parametrize("k", [1, 6])
+@pytest.mark.parametrize("lead", [60.0, 100.0, 150.0, 900.0])
+def test_rest_of_sure_students(cuda, rows, hidden, vocab, k, lead):
+    """The best listed logit stands `lead` above the unlisted ones, whose mass is below what fp32 (88) or fp64 (745) holds: their
+    gradient is that of their own softmax times what the teacher has there."""
+    h, w, t, gen = oracle.make_inputs(rows, hidden, vocab, 7, cuda)
+    ids = torch.stack([torch.randperm(vocab, generator=gen)[:k] for _ in range(rows)]).to(cuda)
+    ids[:, 0] = torch.arange(rows, device=cuda)
+    h = (h.float() + lead / 3 * w[:rows].float()).bfloat16()
+    teacher = torch.randn(rows, k, generator=gen).to(cuda)
+    lse = teacher.logsumexp(1) + 0.3
+    g = torch.randn(rows, generator=gen).to(cuda)
+    want = masses.divergence(h, w, ids, teacher, g, None, lse)
+    h.requires_grad_()
+    w.requires_grad_()
+    loss = K.head_topk_divergence(h, w, ids, teacher, teacher_lse=lse)
+    for got, i in zip((loss.detach(), *torch.autograd.grad(loss, [h, w], g)), (0, 2, 4)):
+        oracle.within(got, want[i], want[i + 1], i)
