@@ -274,7 +274,9 @@ Tensor head_loss(const Tensor& h, const Tensor& weight, const Tensor& ids, const
 }
 
 std::tuple<Tensor, Tensor, Tensor> top_logits(Tensor logits, int64_t k, OptTensor inv_temp) {
-  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.stride(1) == 1, "logits must be 2-D CUDA rows of unit inner stride");
+  // a single column may have any inner stride, contiguous or not
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && (logits.stride(1) == 1 || logits.size(1) == 1),
+              "logits must be 2-D CUDA rows of unit inner stride");
   TORCH_CHECK(logits.scalar_type() == torch::kFloat32 || logits.scalar_type() == torch::kBFloat16, "logits must be fp32 or bf16");
   const int64_t R = logits.size(0), V = logits.size(1);
   TORCH_CHECK(R >= 1 && k >= 1 && k <= V && k <= osb::kTopLogitsMax && V < (1ll << 31) - 65536, "top_logits sizes");

@@ -125,3 +125,15 @@ def test_rest_of_sure_students(cuda, rows, hidden, vocab, k, lead):
     loss = K.head_topk_divergence(h, w, ids, teacher, teacher_lse=lse)
     for got, i in zip((loss.detach(), *torch.autograd.grad(loss, [h, w], g)), (0, 2, 4)):
         oracle.within(got, want[i], want[i + 1], i)
+
+
+@pytest.mark.parametrize("layout", ["transposed", "every_other"])
+def test_one_column_of_any_stride(cuda, layout):
+    """The inner stride of a single column means nothing."""
+    x = torch.randn(5, generator=torch.Generator().manual_seed(1))
+    wide = torch.zeros(5, 6)
+    wide[:, 0] = x
+    logits = x.to(cuda)[None].t() if layout == "transposed" else wide.to(cuda)[:, ::2][:, :1]
+    assert logits.shape == (5, 1) and logits.stride(1) != 1
+    values, ids, lse = K.top_logits(logits, 1)
+    assert torch.equal(values.cpu()[:, 0], x) and not bool(ids.any()) and torch.equal(lse.cpu(), x)
