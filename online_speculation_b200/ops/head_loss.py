@@ -171,8 +171,8 @@ def top_logits(logits: torch.Tensor, k: int, *, inv_temp: torch.Tensor | None = 
 
 # ----------------------------------------------------------------- oracles --
 def _empty_loss(h, weight):
-    """No rows: an empty loss that still reaches its inputs."""
-    return h.float().sum(1) + 0.0 * weight.float().sum()
+    """No rows: an empty loss that still reaches its inputs, and reads none of the head."""
+    return h.float().sum(1) + weight[:0].float().sum()
 
 
 def _scatter_rows(rows, values, count):
