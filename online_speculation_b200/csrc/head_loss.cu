@@ -48,6 +48,12 @@ constexpr int kBN = 256;                  // tile columns: both CTAs hold all of
 constexpr int kHalf = 128;                // rows of A, and of B, that one CTA stages
 constexpr int kBK = 64;                   // reduction elements a stage: one 128-byte swizzle row
 constexpr int kMaxStages = 12;
+// Statistics of many rows: the tensor core truncates at every addition, so a reduction of more than kOneSum blocks is cut
+// into sums of at most kSumBlocks, which the epilogue adds in fp32.  The first two are the longest: while they are
+// multiplied, the exponentials of the tile before are formed.  Divergence losses of 300 rows of 3584, off by 3.8e-6 in one sum:
+// 5.3e-7 (6.2e-7 with fp32 products); the pass over 4096 rows of 3584 and 152064 columns 3.67 ms for 3.50 (sums of 14 blocks 3.60, of 8 3.83).
+// 14 blocks in one sum are off by 9e-7 at most.
+constexpr int kSumBlocks = 10, kOneSum = 14;
 constexpr int kRowBytes = kBK * 2;        // one staged row of either operand
 constexpr int kBox = 64 * 64 * 2;         // one MN-major box: 64 reduction rows of 64 elements
 constexpr int kOutBytes = 32 * 128;       // one warp's staged output box: 32 rows of 128 bytes
@@ -86,6 +92,8 @@ struct GemmArgs {
   int v0, cols;            // this piece: first vocabulary row, columns that exist
   int bn;                  // rows in columns: how many columns, a multiple of 16
   int chains, chain;       // rows in columns: sums of that many blocks of the reduction each, side by side in the accumulator
+  int sums;                // statistics of many rows: sums that the reduction is cut into, added up in registers, and
+  int sum_first, sum_rest; // the blocks of the first two and of the others
   int tiles_n;             // column tiles of the accumulator grid
   int lo;                  // rows in columns: where a row of the logits' gradient holds what rounding to bf16 took
                            // from its first half (0: not kept)
@@ -139,7 +147,7 @@ __host__ __device__ inline StageBytes stage_bytes_of(int mode, bool few, const G
 
 __host__ __device__ inline int out_bytes_of(int mode, bool few, bool kept) {
   if (few && mode == kProd) return 2 * kOutTotal;
-  if (!few) return mode == kStats && !kept ? 0 : kOutTotal;
+  if (!few) return mode == kStats ? (kept ? 2 * kOutTotal : 0) : kOutTotal;
   return (mode == kStats && !kept ? 0 : kOutTotal) + kOutTotal / 2;   // a block for listed logits, behind the boxes
 }
 
@@ -240,6 +248,20 @@ __device__ __forceinline__ void pair_commit(uint64_t* bar) {
 
 __device__ __forceinline__ void remote_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// Adds 32 lanes x 16 accumulator columns (half a load at a time: registers are short where it is used).
+__device__ __forceinline__ void add_tmem16(uint32_t from, float* x) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(from)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] += __uint_as_float(r[i]);
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -444,7 +466,8 @@ __device__ __forceinline__ float* block_at(uint8_t* buf, int row, int col) {
   return reinterpret_cast<float*>(buf + swizzled(row, col >> 2) + (col & 3) * 4);
 }
 
-template <int MODE, bool FEW>
+// SUMS: the reduction is cut into several sums (statistics of many rows).
+template <int MODE, bool FEW, bool SUMS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW), 1)
     head_gemm_kernel(const __grid_constant__ Maps maps, const GemmArgs a) {
   extern __shared__ uint8_t smem_raw[];
@@ -575,47 +598,49 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW
       const uint32_t base = smem_u32(smem);
       Item it;
       for (int i = 0; ok && item_at<MODE, FEW>(a, rows, pair, pairs, i, it); ++i) {
-        if (it.kb0 >= it.kb1) continue;
-        if (!mbar_wait(&tempty[acc], acc_phase ^ 1, a.status, kErrAccumWait)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t d = tmem + acc * kBN;
-        const bool mn_a = MODE == kProd && (it.kind == (FEW ? 0 : 1)), mn_b = MODE == kProd;
-        const int columns = FEW && it.kind == 0 ? (MODE == kProd && a.lo > 0 ? 2 * a.bn : a.bn) : kBN;
-        const uint32_t idesc = idesc_bf16_f32(kBM, columns) | (mn_a ? 1u << 15 : 0u) | (mn_b ? 1u << 16 : 0u);
-        constexpr bool kChains = FEW && MODE != kProd;
-        uint32_t dk = d;
-        int from = it.kb0, turn = a.chain;
-        for (int kb = it.kb0; kb < it.kb1; ++kb) {
-          if (!mbar_wait(&full[stage], phase, a.status, kErrMmaWait)) {
+        for (int n = 0, begin = it.kb0, end; ok && begin < it.kb1; ++n, begin = end) {
+          end = SUMS ? min(begin + (n < 2 ? a.sum_first : a.sum_rest), it.kb1) : it.kb1;
+          if (!mbar_wait(&tempty[acc], acc_phase ^ 1, a.status, kErrAccumWait)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t pa = base + stage * stage_bytes, pb = pa + sb.a;
-          if (kChains && kb == turn) {
-            dk += a.bn;
-            from = kb;
-            turn += a.chain;
-          }
+          const uint32_t d = tmem + acc * kBN;
+          const bool mn_a = MODE == kProd && (it.kind == (FEW ? 0 : 1)), mn_b = MODE == kProd;
+          const int columns = FEW && it.kind == 0 ? (MODE == kProd && a.lo > 0 ? 2 * a.bn : a.bn) : kBN;
+          const uint32_t idesc = idesc_bf16_f32(kBM, columns) | (mn_a ? 1u << 15 : 0u) | (mn_b ? 1u << 16 : 0u);
+          constexpr bool kChains = FEW && MODE != kProd;
+          uint32_t dk = d;
+          int from = begin, turn = a.chain;
+          for (int kb = begin; kb < end; ++kb) {
+            if (!mbar_wait(&full[stage], phase, a.status, kErrMmaWait)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t pa = base + stage * stage_bytes, pb = pa + sb.a;
+            if (kChains && kb == turn) {
+              dk += a.bn;
+              from = kb;
+              turn += a.chain;
+            }
 #pragma unroll
-          for (int k = 0; k < kBK / 16; ++k) {
-            const uint64_t ad = mn_a ? sdesc_mn_sw128(pa + k * 2048, kBox, 1024) : sdesc_k_sw128(pa + k * 32);
-            const uint64_t bd = mn_b ? sdesc_mn_sw128(pb + k * 2048, kBox, 1024) : sdesc_k_sw128(pb + k * 32);
-            pair_mma(dk, ad, bd, idesc, (kb > from || k > 0) ? 1u : 0u);
+            for (int k = 0; k < kBK / 16; ++k) {
+              const uint64_t ad = mn_a ? sdesc_mn_sw128(pa + k * 2048, kBox, 1024) : sdesc_k_sw128(pa + k * 32);
+              const uint64_t bd = mn_b ? sdesc_mn_sw128(pb + k * 2048, kBox, 1024) : sdesc_k_sw128(pb + k * 32);
+              pair_mma(dk, ad, bd, idesc, (kb > from || k > 0) ? 1u : 0u);
+            }
+            pair_commit(&empty[stage]);
+            if (++stage == stages) {
+              stage = 0;
+              phase ^= 1;
+            }
           }
-          pair_commit(&empty[stage]);
-          if (++stage == stages) {
-            stage = 0;
-            phase ^= 1;
-          }
+          if (!ok) break;
+          pair_commit(&tfull[acc]);
+          acc ^= 1;
+          if (acc == 0) acc_phase ^= 1;
         }
-        if (!ok) break;
-        pair_commit(&tfull[acc]);
-        acc ^= 1;
-        if (acc == 0) acc_phase ^= 1;
       }
       // every issued MMA completes before TMEM is released
       pair_commit(drain);
@@ -626,7 +651,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW
     const int quarter = warp % 4;
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
     constexpr int kSets = epilogue_warps(MODE, FEW) / 4;
-    constexpr int kBoxes = FEW ? 2 : 1;                     // output boxes of a warp
+    constexpr int kBoxes = FEW || MODE == kStats ? 2 : 1;                     // output boxes of a warp
     const int set = (warp - 2) / 4;                         // its share of the columns
     uint8_t* out = sOut + (kSets == 1 ? quarter : warp - 2) * kBoxes * kOutBytes;
     auto next_box = [&](int staged) {
@@ -743,14 +768,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW
         c2 = next_scale;
         if (more) fetch_row(ahead);
       }
-      if (!empty_sum) {
-        const bool ok = __all_sync(0xffffffffu, mbar_wait(&tfull[acc], acc_phase, a.status, kErrEpilogueWait));
-        if (!ok) {
-          gave_up = true;
-          if (FEW && MODE != kProd && a.K > 1) continue;   // the other warps still wait for this one above
-          break;
-        }
-        tc_fence_after();
+      auto wait_accumulator = [&]() {
+        gave_up = !__all_sync(0xffffffffu, mbar_wait(&tfull[acc], acc_phase, a.status, kErrEpilogueWait));
+        if (!gave_up) tc_fence_after();
+        return !gave_up;
+      };
+      if (!empty_sum && !wait_accumulator()) {
+        if (FEW && MODE != kProd && a.K > 1) continue;   // the other warps still wait for this one above
+        break;
       }
       const uint32_t t_acc = tmem + lane_base + acc * kBN;
       bool released = false;
@@ -759,6 +784,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW
         __syncwarp();
         if (lane == 0) remote_arrive(map_shared_rank(smem_u32(&tempty[acc]), 0));
         released = true;
+      };
+      auto next_accumulator = [&]() {
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1;
+        released = false;
       };
 
       if (FEW && MODE != kProd) {
@@ -911,15 +941,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW
             ++staged;
           }
         }
-      } else if (MODE == kStats && a.kept) {
-        // the warp's half of the tile in registers, exponentials about its maximum
+      } else if (MODE == kStats && (SUMS || a.kept)) {
+        // the warp's half of the tile in registers: sums added up, then exponentials about its maximum
         float x[kBN / 64][32], plain = 0.0f;
         const int first = it.n0 + set * (kBN / 2);
-        if (m0 < rows) {
-          float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        // the other sums; rows behind the last only let go of them
+        auto next_sum = [&]() {
+          if (!released) release();
+          next_accumulator();
+          return wait_accumulator();
+        };
+        if (m0 >= rows) {
+          for (int n = 1; SUMS && n < a.sums; ++n)
+            if (!next_sum()) break;
+        } else {
 #pragma unroll
           for (int c = 0; c < kBN / 64; ++c) tmem_ld32(t_acc + set * (kBN / 2) + c * 32, x[c]);
           release();
+          for (int n = 1; SUMS && n < a.sums; ++n) {
+            if (!next_sum()) break;
+            const uint32_t from = tmem + lane_base + acc * kBN + set * (kBN / 2);
+#pragma unroll
+            for (int c = 0; c < kBN / 64; ++c) {
+              add_tmem16(from + c * 32, x[c]);
+              add_tmem16(from + c * 32 + 16, x[c] + 16);
+            }
+            release();
+          }
+        }
+        if (SUMS && gave_up) break;
+        if (m0 < rows) {
+          float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
           for (int c = 0; c < kBN / 64; ++c) {
             const int col = first + c * 32;
@@ -953,31 +1005,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW
           const float ref = mx == -INFINITY ? 0.0f : mx;
           const float2 minus = make_float2(-ref, -ref), scale = make_float2(c2, c2), up = make_float2(kKeptOne, kKeptOne);
           float2 s2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+          if (!SUMS || a.kept) {
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            uint8_t* box = next_box(staged);
+            for (int b = 0; b < 2; ++b) {
+              uint8_t* box = next_box(staged);
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-              unsigned packed[4];
+              for (int q = 0; q < 8; ++q) {
+                unsigned packed[4];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float* from = &x[2 * b + q / 4][(q % 4) * 8 + 2 * e];
-                float2 d = mul2(add2(make_float2(from[0], from[1]), minus), scale);
-                d = make_float2(ex2(d.x), ex2(d.y));
-                s2[e & 1] = add2(s2[e & 1], d);
-                d = mul2(d, up);
-                const __half2 h = __floats2half2_rn(d.x, d.y);
-                packed[e] = *reinterpret_cast<const unsigned*>(&h);
+                for (int e = 0; e < 4; ++e) {
+                  const float* from = &x[2 * b + q / 4][(q % 4) * 8 + 2 * e];
+                  float2 d = mul2(add2(make_float2(from[0], from[1]), minus), scale);
+                  d = make_float2(ex2(d.x), ex2(d.y));
+                  s2[e & 1] = add2(s2[e & 1], d);
+                  d = mul2(d, up);
+                  const __half2 h = __floats2half2_rn(d.x, d.y);
+                  packed[e] = *reinterpret_cast<const unsigned*>(&h);
+                }
+                *reinterpret_cast<uint4*>(box + swizzled(lane, q)) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
               }
-              *reinterpret_cast<uint4*>(box + swizzled(lane, q)) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                tma_store_2d(&maps.out0, box, first + b * 64, m0);
+                bulk_commit();
+              }
+              ++staged;
             }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              tma_store_2d(&maps.out0, box, first + b * 64, m0);
-              bulk_commit();
-            }
-            ++staged;
+          } else {
+#pragma unroll
+            for (int c = 0; c < kBN / 64; ++c)
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                const float2 d = mul2(add2(make_float2(x[c][2 * j], x[c][2 * j + 1]), minus), scale);
+                s2[j & 1] = add2(s2[j & 1], make_float2(ex2(d.x), ex2(d.y)));
+              }
           }
           if (live) {
             const long long p = static_cast<long long>(m) * a.part_tiles + 2 * (it.n0 / kBN) + set;
@@ -1167,8 +1229,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW
       if (!FEW && MODE != kProd && more) fetch_id();
       if (!empty_sum) {
         if (!released) release();
-        acc ^= 1;
-        if (acc == 0) acc_phase ^= 1;
+        next_accumulator();
       }
     }
     if (FEW && MODE == kStats) {
@@ -1423,7 +1484,7 @@ __global__ void __launch_bounds__(128) gather_rows_kernel(const HeadLossState s)
 // The tensor core's sums of H products come out a little short (its additions truncate: about 2e-6 of a
 // logit at H = 3584 in one chain).  Listed logits and normaliser share that, so most of it cancels in a loss; listed
 // logits summed again in fp32 made the losses worse (1.2e-6 for 0.9e-6 relative, 64 rows of 152064).  Up to 128
-// rows have room for several chains (2.0e-7, at no time).
+// rows have room for several chains (2.0e-7, at no time); more than 256 are summed in parts (kSumBlocks).
 __global__ void __launch_bounds__(128) finish_rows_kernel(const HeadLossState s, const HeadStatsScratch p) {
   __shared__ double buf_d[4];
   __shared__ float buf_f[4];
@@ -1779,14 +1840,14 @@ int lane_slot(int cols, int step) {
   return best;
 }
 
-template <int MODE, bool FEW>
+template <int MODE, bool FEW, bool SUMS = false>
 cudaError_t launch_gemm(const Maps& maps, GemmArgs a, int max_items, cudaStream_t stream) {
   static bool set[64] = {false};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev >= 64 || !set[dev]) {
-    e = cudaFuncSetAttribute(head_gemm_kernel<MODE, FEW>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost + 1024);
+    e = cudaFuncSetAttribute(head_gemm_kernel<MODE, FEW, SUMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost + 1024);
     if (e != cudaSuccess) return e;
     if (dev < 64) set[dev] = true;
   }
@@ -1794,7 +1855,7 @@ cudaError_t launch_gemm(const Maps& maps, GemmArgs a, int max_items, cudaStream_
   const StageBytes sb = stage_bytes_of(MODE, FEW, a);
   a.stages = std::min(kMaxStages, (kSmemMost - rest) / (sb.a + sb.b));
   const int smem = 1024 + a.stages * (sb.a + sb.b) + rest;
-  return launch_pdl(head_gemm_kernel<MODE, FEW>, dim3(2 * pairs_for(max_items)), dim3(threads_of(MODE, FEW)), smem, stream, maps, a);
+  return launch_pdl(head_gemm_kernel<MODE, FEW, SUMS>, dim3(2 * pairs_for(max_items)), dim3(threads_of(MODE, FEW)), smem, stream, maps, a);
 }
 
 GemmArgs base_args(const HeadLossState& s) {
@@ -1812,6 +1873,12 @@ GemmArgs base_args(const HeadLossState& s) {
   // us where chains of neighbours take 226 (64 rows of 3584 on 152064 columns).
   a.chain = ceil_div(ceil_div(s.H, kBK), most_chains(a.bn));
   a.chains = ceil_div(ceil_div(s.H, kBK), a.chain);
+  // the issuer makes as many sums as the epilogue takes: two of sum_first blocks, others of sum_rest, none empty
+  const int blocks = ceil_div(s.H, kBK);
+  a.sum_first = blocks <= kOneSum ? blocks : std::min(kSumBlocks, ceil_div(blocks, 2));
+  const int others = ceil_div(std::max(blocks - 2 * a.sum_first, 0), kSumBlocks);
+  a.sum_rest = others > 0 ? ceil_div(blocks - 2 * a.sum_first, others) : 1;
+  a.sums = std::min(blocks, 2 * a.sum_first) > a.sum_first ? 2 + others : 1;
   a.lo = s.R <= kSplitRows ? ceil_div(s.R, 64) * 64 : 0;
   a.status = s.status;
   return a;
@@ -1932,7 +1999,8 @@ cudaError_t head_loss_forward_launch(const HeadLossState& s, const HeadStatsScra
     a.kept = p.kept != nullptr;
     const int pitch = head_loss_kept(s.R, s.H, s.V).pitch;
     if (a.kept && !map_bf16(&maps.out0, p.kept, s.rpad, pitch, pitch, 64, 32)) return cudaErrorInvalidValue;   // fp16
-    e = launch_gemm<kStats, false>(maps, a, ceil_div(s.R, kBM) * a.tiles_n, stream);
+    const int items = ceil_div(s.R, kBM) * a.tiles_n;
+    e = a.sums > 1 ? launch_gemm<kStats, false, true>(maps, a, items, stream) : launch_gemm<kStats, false>(maps, a, items, stream);
   }
   if (e != cudaSuccess) return e;
   return launch_pdl(finish_rows_kernel, dim3(s.R), dim3(128), 0, stream, s, p);

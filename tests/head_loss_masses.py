@@ -23,18 +23,22 @@ import head_loss_oracle as oracle
 
 def losses(h, w, ids, teacher, inv_temp=None, teacher_lse=None):
     """(loss, what the gradient needs) in the type of ``h`` and ``w``, differentiable."""
-    vocab = w.shape[0]
+    return losses_of_logits(h @ w.t(), ids, teacher, inv_temp, teacher_lse)
+
+
+def losses_of_logits(logits, ids, teacher, inv_temp=None, teacher_lse=None):
+    vocab = logits.shape[1]
     slot = (ids >= 0) & (teacher != -math.inf)
-    it = h.new_ones(h.shape[0]) if inv_temp is None else inv_temp.to(h.dtype)
-    z = (teacher.to(h.dtype) * it[:, None]).masked_fill(~slot, -math.inf)
+    it = logits.new_ones(logits.shape[0]) if inv_temp is None else inv_temp.to(logits.dtype)
+    z = (teacher.to(logits.dtype) * it[:, None]).masked_fill(~slot, -math.inf)
     spot = torch.where(slot, ids.long(), vocab)
     some = slot.any(1)
-    norm = torch.where(some, z.logsumexp(1), 0.0) if teacher_lse is None else teacher_lse.to(h.dtype)
-    p = h.new_zeros(h.shape[0], vocab + 1).scatter_add_(1, spot, (z - norm[:, None]).exp())[:, :-1]
-    on = torch.zeros(p.shape[0], vocab + 1, dtype=torch.bool, device=h.device).scatter_(1, spot, True)[:, :-1]
+    norm = torch.where(some, z.logsumexp(1), 0.0) if teacher_lse is None else teacher_lse.to(logits.dtype)
+    p = logits.new_zeros(logits.shape[0], vocab + 1).scatter_add_(1, spot, (z - norm[:, None]).exp())[:, :-1]
+    on = torch.zeros(p.shape[0], vocab + 1, dtype=torch.bool, device=logits.device).scatter_(1, spot, True)[:, :-1]
     total, whole = p.sum(1), on.all(1)
     rest = torch.where(whole | ~some, 0.0, (1 - total).clamp_min(0)) if teacher_lse is not None else torch.zeros_like(total)
-    log_q = ((h @ w.t()) * it[:, None]).log_softmax(1)
+    log_q = (logits * it[:, None]).log_softmax(1)
     log_rest = log_q.masked_fill(on & ~whole[:, None], -math.inf).logsumexp(1)
     part = torch.where(p > 0, p * (torch.where(p > 0, p, 1.0).log() - log_q), 0.0).sum(1)
     part = part + torch.where(rest > 0, rest * (torch.where(rest > 0, rest, 1.0).log() - log_rest), 0.0)
