@@ -24,11 +24,11 @@
 //   Both read dl and their other operand in the layout they already have (MN-major
 //   shared-memory descriptors): nothing is transposed.  What rounding took from the listed entries is added to dh
 //   on its way out, where the list is short against the vocabulary (hidden_grad_kernel).
-// * Up to 256 rows take the products the other way around, vocabulary columns in the accumulator's
+// * Up to 128 rows take the products the other way around, vocabulary columns in the accumulator's
 //   lanes and rows in its columns.  A pass over few rows is the reading of the head, and a tile of
 //   256 lanes that holds 64 rows would spend four times the matrix instructions (and the clock that
 //   their power costs: 93 % tensor-pipe active at 1.5 GHz for 64 rows) on lanes that nobody looks at.
-// * Up to 128 rows keep dl as the sum of two bf16 numbers.  A row's gradient is mostly its target's
+// * They keep dl as the sum of two bf16 numbers.  A row's gradient is mostly its target's
 //   entry: with few rows the rounding of single entries shows in the results (0.0027 relative where the
 //   rounding of the outputs alone is 0.0017), and the second half is nearly free, as the head is read
 //   all the same.  With many rows the errors average out and the products would double.
@@ -63,8 +63,8 @@ constexpr int kOutBytes = 32 * 128;       // one warp's staged output box: 32 ro
 constexpr int epilogue_warps(int mode, bool few) { return few && mode != 2 ? 4 : 8; }
 constexpr int threads_of(int mode, bool few) { return 64 + 32 * epilogue_warps(mode, few); }   // and TMA, MMA
 constexpr int kOutTotal = 8 * kOutBytes;  // two boxes a warp, or one with twice the warps
-constexpr int kFewRows = 256;             // rows that fit the accumulator's columns
-constexpr int kSplitRows = 128;           // rows whose logits' gradient is kept in two bf16 halves
+constexpr int kFewRows = 128;             // rows that go into the accumulator's columns: see few_rows
+constexpr int kCountRows = 256;           // rows that one launch numbers and gathers
 // Per-row state of the passes with rows in columns, behind the output boxes: running maximum and sum and
 // plain sum (one set a warp), list cursors (one set a warp, two of the CTA), coefficients, row numbers, targets' gradients.
 constexpr int kStateMax = 0, kStateSum = kStateMax + 4 * kFewRows * 4, kStatePlain = kStateSum + 4 * kFewRows * 4,
@@ -96,7 +96,7 @@ struct GemmArgs {
   int sum_first, sum_rest; // the blocks of the first two and of the others
   int tiles_n;             // column tiles of the accumulator grid
   int lo;                  // rows in columns: where a row of the logits' gradient holds what rounding to bf16 took
-                           // from its first half (0: not kept)
+                           // from its first half
   int slot;                // rows in columns: vocabulary columns in the lanes of one CTA (statistics: a multiple of
                            // 8, gradient: of 32)
   int stages;              // of the ring
@@ -118,9 +118,8 @@ struct GemmArgs {
   int* status;
 };
 
-// Rows in columns, hidden gradient: boxes of 64 rows that one CTA stages, its half of the rows or, in two
-// halves, all rows of one of them.
-__host__ __device__ inline int row_boxes(const GemmArgs& a) { return ((a.lo > 0 ? a.bn : a.bn / 2) + 63) / 64; }
+// Rows in columns, hidden gradient: boxes of 64 rows that one CTA stages, all rows of one of the two halves.
+__host__ __device__ inline int row_boxes(const GemmArgs& a) { return (a.bn + 63) / 64; }
 
 // Rows in columns: columns of the accumulator, and the most chains of a sum that stand in it side by side.
 __host__ __device__ constexpr int row_columns(int R) { return (R + 15) / 16 * 16; }
@@ -183,7 +182,7 @@ __device__ __forceinline__ bool item_at(const GemmArgs& a, int rows, int pair, i
   // The hidden gradient's items reduce over the piece, the head gradient's over the rows, and cost
   // accordingly: the former go first, dealt around; the pairs that got one less take as many of the
   // latter in its place as weigh the same, and the rest is dealt around.
-  const int kb = (a.cols + kBK - 1) / kBK, per = (kb + a.splits - 1) / a.splits, kbw = (rows + kBK - 1) / kBK * (FEW && a.lo > 0 ? 2 : 1);
+  const int kb = (a.cols + kBK - 1) / kBK, per = (kb + a.splits - 1) / a.splits, kbw = (rows + kBK - 1) / kBK * (FEW ? 2 : 1);
   const int per_split = FEW ? (rows > 0 ? a.tiles_n : 0) : tm * a.tiles_n;   // a.tiles_n tiles across the hidden width
   const int nh = a.do_dh ? per_split * a.splits : 0;
   const int nw = a.do_dw ? ((a.cols + kBM - 1) / kBM) * a.tiles_n : 0;
@@ -368,32 +367,17 @@ struct ListCursor {
   }
 };
 
-// Where the lists of all rows reach `col`, and the first column there: each of the 128 epilogue threads takes two
-// rows, whose searches go on side by side.  (Every warp on its own, its lanes one row after the other, took
-// longer than a tile of 64 hidden columns with 256 rows.)
+// Where the lists of all rows reach `col`, and the first column there: a row for each of the 128 epilogue threads.
+// (Every warp on its own, its lanes one row after the other, took longer than a tile of 64 hidden columns with 256 rows.)
 __device__ __forceinline__ void seek_rows(const int* list_id, int K, const int* row_no, int rows, int col, int2* cursors) {
-  constexpr int kEach = kFewRows / 128;
-  const int t0 = threadIdx.x - 64;
-  const int* ids[kEach];
-  int lo[kEach], id[kEach];
-#pragma unroll
-  for (int j = 0; j < kEach; ++j) {
-    ids[j] = list_id + static_cast<long long>(row_no[min(t0 + j * 128, rows - 1)]) * K;
-    lo[j] = 0;
-  }
-  int top = 1;
+  static_assert(kFewRows == 128, "a thread a row");
+  const int t = threadIdx.x - 64;
+  if (t >= rows) return;
+  const int* ids = list_id + static_cast<long long>(row_no[t]) * K;
+  int at = 0, top = 1;
   while (2 * top <= K) top *= 2;
-  for (int step = top; step > 0; step /= 2) {
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) id[j] = ids[j][min(lo[j] + step, K) - 1];
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) lo[j] += lo[j] + step <= K && id[j] < col ? step : 0;
-  }
-#pragma unroll
-  for (int j = 0; j < kEach; ++j) id[j] = ids[j][min(lo[j], K - 1)];
-#pragma unroll
-  for (int j = 0; j < kEach; ++j)
-    if (t0 + j * 128 < rows) cursors[t0 + j * 128] = make_int2(lo[j], lo[j] < K ? id[j] : INT_MAX);
+  for (int step = top; step > 0; step /= 2) at += at + step <= K && ids[at + step - 1] < col ? step : 0;
+  cursors[t] = make_int2(at, at < K ? ids[at] : INT_MAX);
 }
 
 // A row's coefficients of the logits' gradient: {it log2 e, lse log2 e, A, C} of A exp(it l - lse) - C.  A divergence's are
@@ -552,10 +536,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW
             for (int j = 0; j < kHalf / 64; ++j)
               pair_load_2d(pa + j * kBox, &maps.a0, it.m0 + rank * kHalf + j * 64, a.v0 + k0, bar);
             for (int j = 0; j < rows_box; ++j)
-              pair_load_2d(pb + j * kBox, &maps.b0, rank * (a.lo > 0 ? a.lo : a.bn / 2) + j * 64, k0, bar);
+              pair_load_2d(pb + j * kBox, &maps.b0, rank * a.lo + j * 64, k0, bar);
           } else {
             // head gradient in two halves: the second half's blocks meet the same rows again
-            const int over = k0 - (FEW && a.lo > 0 ? (rows + kBK - 1) / kBK * kBK : INT_MAX);
+            const int over = k0 - (FEW ? (rows + kBK - 1) / kBK * kBK : INT_MAX);
             const int ka = over >= 0 ? a.lo + over : k0, kh = over >= 0 ? over : k0;
             const int ma = it.m0 + rank * kHalf, nb = it.n0 + rank * kHalf;
             if (MODE != kProd) {
@@ -607,7 +591,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW
           tc_fence_after();
           const uint32_t d = tmem + acc * kBN;
           const bool mn_a = MODE == kProd && (it.kind == (FEW ? 0 : 1)), mn_b = MODE == kProd;
-          const int columns = FEW && it.kind == 0 ? (MODE == kProd && a.lo > 0 ? 2 * a.bn : a.bn) : kBN;
+          const int columns = FEW && it.kind == 0 ? (MODE == kProd ? 2 * a.bn : a.bn) : kBN;
           const uint32_t idesc = idesc_bf16_f32(kBM, columns) | (mn_a ? 1u << 15 : 0u) | (mn_b ? 1u << 16 : 0u);
           constexpr bool kChains = FEW && MODE != kProd;
           uint32_t dk = d;
@@ -877,13 +861,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW
             sums[t] = sums[t] * kept + s;
             __syncwarp();
           } else {
-            // one box at a time in turn, or both for the two halves
-            uint8_t* box = out + (a.lo > 0 ? 0 : (staged & 1) * kOutBytes);
+            // a box for either half
+            uint8_t* box = out;
             if ((c & 1) == 0) {
-              if (lane == 0) {
-                if (a.lo > 0) bulk_wait_read<0>();
-                else bulk_wait_read<1>();
-              }
+              if (lane == 0) bulk_wait_read<0>();
               __syncwarp();
             }
 #pragma unroll
@@ -906,17 +887,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW
               const uint4 v = make_uint4(pack2(x[8 * q], x[8 * q + 1]), pack2(x[8 * q + 2], x[8 * q + 3]),
                                          pack2(x[8 * q + 4], x[8 * q + 5]), pack2(x[8 * q + 6], x[8 * q + 7]));
               *reinterpret_cast<uint4*>(box + swizzled(lane, (c & 1) * 4 + q)) = on ? v : make_uint4(0, 0, 0, 0);
-              if (a.lo > 0) {
-                const uint4 low = rounded_off(x + 8 * q, v);
-                *reinterpret_cast<uint4*>(box + kOutBytes + swizzled(lane, (c & 1) * 4 + q)) = on ? low : make_uint4(0, 0, 0, 0);
-              }
+              const uint4 low = rounded_off(x + 8 * q, v);
+              *reinterpret_cast<uint4*>(box + kOutBytes + swizzled(lane, (c & 1) * 4 + q)) = on ? low : make_uint4(0, 0, 0, 0);
             }
             if (c & 1) {
               fence_proxy_async_smem();
               __syncwarp();
               if (lane == 0) {
                 tma_store_2d(&maps.out0, box, (c >> 1) * 64, m0);
-                if (a.lo > 0) tma_store_2d(&maps.out0, box + kOutBytes, a.lo + (c >> 1) * 64, m0);
+                tma_store_2d(&maps.out0, box + kOutBytes, a.lo + (c >> 1) * 64, m0);
                 bulk_commit();
               }
               ++staged;
@@ -935,7 +914,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW
             __syncwarp();
             if (lane == 0) {
               tma_store_2d(&maps.out0, box, c * 64, m0);
-              if (a.lo > 0) tma_store_2d(&maps.out0, box, a.lo + c * 64, m0);
+              tma_store_2d(&maps.out0, box, a.lo + c * 64, m0);
               bulk_commit();
             }
             ++staged;
@@ -1149,12 +1128,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW
         for (int c = set; c < (rows + 31) / 32 && m0 < a.H; c += kSets) {
           float x[32];
           tmem_ld32(t_acc + c * 32, x);
-          if (a.lo > 0) {
-            float y[32];
-            tmem_ld32(t_acc + a.bn + c * 32, y);
+          float y[32];
+          tmem_ld32(t_acc + a.bn + c * 32, y);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) x[j] += y[j];
-          }
+          for (int j = 0; j < 32; ++j) x[j] += y[j];
           uint8_t* box = next_box(staged);
 #pragma unroll
           for (int j = 0; j < 32; ++j) *block_at(box, j, lane) = x[j];
@@ -1423,7 +1400,7 @@ __global__ void __launch_bounds__(128) few_rows_kernel(const HeadLossState s, co
     return v != t.ignore_index && v >= 0 && v < s.V;
   };
   int before = 0, total = 0;
-  for (int r0 = warp * 32; r0 < kFewRows; r0 += 128) {
+  for (int r0 = warp * 32; r0 < kCountRows; r0 += 128) {
     const unsigned on = __ballot_sync(0xffffffffu, counts(r0 + lane));
     total += __popc(on);
     before += r0 + 32 <= b ? __popc(on) : r0 < b ? __popc(on & ((1u << (b - r0)) - 1u)) : 0;
@@ -1484,7 +1461,7 @@ __global__ void __launch_bounds__(128) gather_rows_kernel(const HeadLossState s)
 // The tensor core's sums of H products come out a little short (its additions truncate: about 2e-6 of a
 // logit at H = 3584 in one chain).  Listed logits and normaliser share that, so most of it cancels in a loss; listed
 // logits summed again in fp32 made the losses worse (1.2e-6 for 0.9e-6 relative, 64 rows of 152064).  Up to 128
-// rows have room for several chains (2.0e-7, at no time); more than 256 are summed in parts (kSumBlocks).
+// rows have room for several chains (2.0e-7, at no time); more are summed in parts (kSumBlocks).
 __global__ void __launch_bounds__(128) finish_rows_kernel(const HeadLossState s, const HeadStatsScratch p) {
   __shared__ double buf_d[4];
   __shared__ float buf_f[4];
@@ -1642,7 +1619,7 @@ __global__ void __launch_bounds__(256, 2) kept_grad_kernel(const HeadLossState s
       const uint4 hi = make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7]));
       __nv_bfloat16* dst = g.dl + static_cast<long long>(v) * pitch + t0;
       *reinterpret_cast<uint4*>(dst) = hi;
-      if (lo > 0) *reinterpret_cast<uint4*>(dst + lo) = rounded_off(x, hi);
+      *reinterpret_cast<uint4*>(dst + lo) = rounded_off(x, hi);
     }
   }
 }
@@ -1722,13 +1699,14 @@ __global__ void __launch_bounds__(128) kept_listed_kernel(const HeadLossState s,
     const __nv_bfloat16 hi = __float2bfloat16_rn(x);
     __nv_bfloat16* dst = g.dl + static_cast<long long>(id - v0) * pitch + m;
     *dst = hi;
-    if (lo > 0) dst[lo] = __float2bfloat16_rn(x - __bfloat162float(hi));
+    dst[lo] = __float2bfloat16_rn(x - __bfloat162float(hi));
   }
 }
 
 // Sums the parts of the hidden gradient.  `mend`: dl had its listed entries, which are most of a row's gradient, in
 // one bf16 number; what rounding took from them times their head rows comes on top here.  (Relative error
-// of dh for a loss with one target 0.0024 without, 0.0017 with it: that of rounding dh itself.)
+// of dh for a loss with one target 0.0024 without, 0.0017 with it: that of rounding dh itself.)  Few rows have
+// those entries in dl's second half.
 constexpr int kMendAhead = 16;   // 192 rows of 3584, lists of 64: 40 us; 8 left to the compiler 64 us
 
 __global__ void __launch_bounds__(128) hidden_grad_kernel(const HeadLossState s, const HeadGradArgs g, int mend) {
@@ -1821,6 +1799,10 @@ int ceil_div(long long a, long long b) { return static_cast<int>((a + b - 1) / b
 // CTA pairs of a launch.
 int pairs_for(int items) { return std::max(1, std::min(items, device_sms() / 2)); }
 
+// Rows in columns, and two such sums in chains, fit up to 128 rows.  More would fit in one chain, three times as far off, and
+// without a second half of dl.  In columns / with the many rows, forward pass and with hidden gradient: 129 rows of 3584 and
+// 152064 columns 239 / 251, 502 / 516 us; 192 rows 278 / 282, 625 / 602; 256 rows 303 / 286, 692 / 625; 136 rows of
+// 896 and 65536 columns 46 / 41, 119 / 99; 192 rows of 512 and 2048 columns 20 / 18, 74 / 78.
 bool few_rows(int R) { return R <= kFewRows; }
 
 // Rows in columns: how many vocabulary columns one CTA's lanes hold, a multiple of `step`.  As many tiles as
@@ -1879,7 +1861,7 @@ GemmArgs base_args(const HeadLossState& s) {
   const int others = ceil_div(std::max(blocks - 2 * a.sum_first, 0), kSumBlocks);
   a.sum_rest = others > 0 ? ceil_div(blocks - 2 * a.sum_first, others) : 1;
   a.sums = std::min(blocks, 2 * a.sum_first) > a.sum_first ? 2 + others : 1;
-  a.lo = s.R <= kSplitRows ? ceil_div(s.R, 64) * 64 : 0;
+  a.lo = ceil_div(s.R, 64) * 64;
   a.status = s.status;
   return a;
 }
@@ -1887,10 +1869,10 @@ GemmArgs base_args(const HeadLossState& s) {
 }  // namespace
 
 // What a forward pass keeps for its backward pass.  Few rows: a logit kept is 8 bytes, written and read, and saves the
-// second reading of the head with its products.  Forward and hidden gradient, kept against computed again: 192 rows
-// of 3584 and 152064 columns 554 / 851 us, 16 rows of 3584 426 / 582 us, 128 rows of 512 174 / 185 us, 256 rows of
-// 64 218 / 215 us; 128 rows of 896 and 32768 columns 75 / 80 us, 64 rows of 512 and 20000 columns 74 / 72 us (one more
-// launch and allocation).  At most 256 MB, and at most twice the head.
+// second reading of the head with its products.  Forward and hidden gradient, kept against computed again: 16 rows
+// of 3584 and 152064 columns 426 / 582 us, 128 rows of 512 174 / 185 us; 128 rows of 896 and 32768 columns
+// 75 / 80 us, 64 rows of 512 and 20000 columns 74 / 72 us (one more launch and allocation).  At most 256 MB, and at most
+// twice the head.
 //
 // Many rows: 4 bytes a logit for 2 H operations.  Both gradients: 4096 rows of 3584 and 152064 columns 9.6 / 11.9 ms, 300
 // rows of 3584 1449 / 1832 us, 1024 rows of 512 and 50000 columns 214 / 228 us, 4096 rows of 256 and 152064
@@ -1916,11 +1898,10 @@ int head_loss_vocab_tiles(int R, int V, bool kept) {
   return few_rows(R) ? 8 * pairs_for(ceil_div(V, 2 * lane_slot(V, kept ? 32 : 8))) : 2 * ceil_div(V, kBN);
 }
 
-// Row pitch or row count of the logits' gradient: [piece][few rows, in two halves up to kSplitRows] or
+// Row pitch or row count of the logits' gradient: [piece][few rows, in two halves] or
 // [rows][piece].
 int head_loss_grad_rows(int R) {
-  if (R <= kSplitRows) return 2 * ceil_div(R, 64) * 64;
-  return few_rows(R) ? ceil_div(R, 64) * 64 : ceil_div(R, kHeadRowPad) * kHeadRowPad;
+  return few_rows(R) ? 2 * ceil_div(R, 64) * 64 : ceil_div(R, kHeadRowPad) * kHeadRowPad;
 }
 
 // Columns of the logits that the backward pass works on at a time.  Their gradient takes two bytes a row and
@@ -1938,7 +1919,7 @@ int head_loss_splits(int R, int H, int piece, int V, bool with_dw) {
   const int pairs = device_sms() / 2, cols = std::min(piece, V), kb = ceil_div(cols, kBK);
   const bool few = few_rows(R);
   const long long tiles = static_cast<long long>(few ? 1 : ceil_div(R, kBM)) * ceil_div(H, kBN);
-  const long long kbw = std::max(ceil_div(R, kBK) * (R <= kSplitRows ? 2 : 1), 8);     // weights: see item_at
+  const long long kbw = std::max(ceil_div(R, kBK) * (few ? 2 : 1), 8);     // weights: see item_at
   const long long other = static_cast<long long>(ceil_div(cols, kBM)) * ceil_div(H, kBN) * kbw;
   const long long bytes = 4ll * ceil_div(R, kHeadRowPad) * kHeadRowPad * H;             // of one partial sum
   int best = 1;
@@ -1964,7 +1945,7 @@ cudaError_t head_loss_rows_launch(const HeadLossState& s, const HeadTargets& t, 
     e = launch_pdl(teacher_rows_kernel, dim3(s.R), dim3(128), 0, stream, s, t);
     if (e != cudaSuccess) return e;
   }
-  if (few_rows(s.R)) return launch_pdl(few_rows_kernel, dim3(s.rpad), dim3(128), 0, stream, s, t);
+  if (s.R <= kCountRows) return launch_pdl(few_rows_kernel, dim3(s.rpad), dim3(128), 0, stream, s, t);
   e = launch_pdl(compact_rows_kernel, dim3(1), dim3(1024), 0, stream, s, t);
   if (e != cudaSuccess) return e;
   return launch_pdl(gather_rows_kernel, dim3(s.rpad), dim3(128), 0, stream, s);
@@ -2075,8 +2056,9 @@ cudaError_t head_loss_backward_launch(const HeadLossState& s, const HeadGradArgs
     if (e != cudaSuccess) return e;
   }
   if (dh) {
-    // reading the listed head rows again: 2 K H bytes a row, next to 4 or 6 H V operations at least
-    const int mend = base.lo == 0 && s.K <= std::max(1, s.V / (few ? 1024 : 4096));
+    // reading the listed head rows again: 2 K H bytes a row, next to 4 or 6 H V operations at least; up to 256 rows the
+    // products take as long as one row tile's
+    const int mend = !few && s.K <= std::max(1, s.V / (s.R <= 256 ? 1024 : 4096));
     return launch_pdl(hidden_grad_kernel, dim3(s.R, ceil_div(s.H, 1024)), dim3(128), 0, stream, s, g, mend);
   }
   return cudaSuccess;

@@ -75,11 +75,12 @@ def head_cross_entropy(h: torch.Tensor, weight: torch.Tensor, targets: torch.Ten
     its row is ignored and ``workspace.check_status`` reports it.  Gradients are bf16, summed in
     fp32.
 
-    Between the passes a step keeps 2 bytes a logit (``2 R V``, up to 2 GB; H at least 384) or, of at most
-    256 (and H) rows on 32768 columns or more, 4 bytes (up to 256 MB); larger ones, and all others,
-    keep nothing and compute the logits twice.  ``piece`` (a multiple of 256) bounds the memory: nothing is
-    kept, and the backward pass works on that many vocabulary columns at a time with ``2 R piece`` bytes
-    of scratch (twice that up to 128 rows; 256 MB without it).
+    Between the passes a step keeps its hidden rows and 2 bytes a logit (up to 2 GB; rows in whole 256; H at least
+    384) or, of at most 128 (and H) rows on 32768 columns or more, 4 bytes (up to 256 MB); larger ones, and
+    all others, keep no logits and compute them twice.  ``piece`` (a multiple of 256) bounds the memory: no logits
+    are kept, and the backward pass works on that many vocabulary columns at a time with ``2 R piece`` bytes
+    of scratch (twice that up to 128 rows; 256 MB without it), next to 4 bytes an entry of ``h`` for each part
+    of its gradient.
 
     A training step that is captured into a CUDA graph takes its gradients with
     ``torch.autograd.grad``; no eager graph of the same leaves may be alive meanwhile.
