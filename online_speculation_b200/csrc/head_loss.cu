@@ -92,7 +92,7 @@ struct GemmArgs {
   int v0, cols;            // this piece: first vocabulary row, columns that exist
   int bn;                  // rows in columns: how many columns, a multiple of 16
   int chains, chain;       // rows in columns: sums of that many blocks of the reduction each, side by side in the accumulator
-  int sums;                // statistics of many rows: sums that the reduction is cut into, added up in registers, and
+  int sums;                // statistics: sums that the reduction is cut into one after the other, added up in registers, and
   int sum_first, sum_rest; // the blocks of the first two and of the others
   int tiles_n;             // column tiles of the accumulator grid
   int lo;                  // rows in columns: where a row of the logits' gradient holds what rounding to bf16 took
@@ -450,7 +450,7 @@ __device__ __forceinline__ float* block_at(uint8_t* buf, int row, int col) {
   return reinterpret_cast<float*>(buf + swizzled(row, col >> 2) + (col & 3) * 4);
 }
 
-// SUMS: the reduction is cut into several sums (statistics of many rows).
+// SUMS: the reduction is cut into several sums (statistics).
 template <int MODE, bool FEW, bool SUMS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW), 1)
     head_gemm_kernel(const __grid_constant__ Maps maps, const GemmArgs a) {
@@ -595,7 +595,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW
           const uint32_t idesc = idesc_bf16_f32(kBM, columns) | (mn_a ? 1u << 15 : 0u) | (mn_b ? 1u << 16 : 0u);
           constexpr bool kChains = FEW && MODE != kProd;
           uint32_t dk = d;
-          int from = begin, turn = a.chain;
+          int from = begin, turn = begin + a.chain;
           for (int kb = begin; kb < end; ++kb) {
             if (!mbar_wait(&full[stage], phase, a.status, kErrMmaWait)) {
               ok = false;
@@ -801,22 +801,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW
           reload_block(buf, x);
         };
         const int chunks = MODE == kStats ? (rows + 31) / 32 : 2 * ((rows + 63) / 64);
-        for (int c = 0; c < chunks && first < stop; ++c) {
+        auto work_on = [&](int c, float (&x)[32]) {
           const int t0 = c * 32, t = t0 + lane;
-          float x[32];
-          if (t0 < rows) {
-            tmem_ld32(t_acc + t0, x);
-            for (int n = 1; n < a.chains; ++n) {
-              float y[32];
-              tmem_ld32(t_acc + n * a.bn + t0, y);
-#pragma unroll
-              for (int j = 0; j < 32; ++j) x[j] += y[j];
-            }
-          } else {
-            // the half of the last box behind the rows: the last chain's columns would end behind the accumulator
-#pragma unroll
-            for (int j = 0; j < 32; ++j) x[j] = 0.0f;
-          }
           if (MODE == kStats) {
             if (a.kept) {
               // lanes outside the vocabulary are cut off by the map: a warp's columns are its own (see lane_slot)
@@ -900,6 +886,60 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE, FEW
               }
               ++staged;
             }
+          }
+        };
+        if (SUMS) {
+          // all rows' sums first, so that the accumulator is soon let go of
+          float x[kFewRows / 32][32];
+          for (int n = 0; n < a.sums; ++n) {
+            if (n > 0) {
+              release();
+              next_accumulator();
+              if (!wait_accumulator()) break;
+            }
+            const uint32_t from = tmem + lane_base + acc * kBN;
+            const int blocks = min(a.sum_rest, it.kb1 - n * a.sum_rest), chains = (blocks + a.chain - 1) / a.chain;
+            for (int k = 0; k < chains; ++k) {
+#pragma unroll
+              for (int c = 0; c < kFewRows / 32; ++c) {
+                if (c * 32 >= rows || first >= stop) break;
+                if (n == 0 && k == 0) {
+                  tmem_ld32(from + c * 32, x[c]);
+                } else {
+                  add_tmem16(from + k * a.bn + c * 32, x[c]);
+                  add_tmem16(from + k * a.bn + c * 32 + 16, x[c] + 16);
+                }
+              }
+            }
+          }
+          if (gave_up) {
+            if (a.K > 1) continue;   // as above
+            break;
+          }
+          release();
+#pragma unroll
+          for (int c = 0; c < kFewRows / 32; ++c) {
+            if (c * 32 >= rows || first >= stop) break;
+            work_on(c, x[c]);
+          }
+        } else {
+          for (int c = 0; c < chunks && first < stop; ++c) {
+            const int t0 = c * 32;
+            float x[32];
+            if (t0 < rows) {
+              tmem_ld32(t_acc + t0, x);
+              for (int n = 1; n < a.chains; ++n) {
+                float y[32];
+                tmem_ld32(t_acc + n * a.bn + t0, y);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) x[j] += y[j];
+              }
+            } else {
+              // the half of the last box behind the rows: the last chain's columns would end behind the accumulator
+#pragma unroll
+              for (int j = 0; j < 32; ++j) x[j] = 0.0f;
+            }
+            work_on(c, x);
           }
         }
         if (MODE == kGrad && first >= stop && quarter * 32 < held && m0 < a.piece) {
@@ -1840,6 +1880,26 @@ cudaError_t launch_gemm(const Maps& maps, GemmArgs a, int max_items, cudaStream_
   return launch_pdl(head_gemm_kernel<MODE, FEW, SUMS>, dim3(2 * pairs_for(max_items)), dim3(threads_of(MODE, FEW)), smem, stream, maps, a);
 }
 
+// Cuts the reduction of the statistics into sums (GemmArgs::sums): as many as the issuer makes of these numbers, none
+// empty.  With rows in columns a sum is as long as its chains allow.
+void cut_sums(GemmArgs& a, bool few) {
+  const int blocks = ceil_div(a.H, kBK);
+  a.sums = 1;
+  a.sum_first = a.sum_rest = blocks;
+  if (few) {
+    if (a.chain <= kOneSum) return;
+    const int chains = most_chains(a.bn);
+    a.sum_first = a.sum_rest = ceil_div(blocks, ceil_div(blocks, chains * kOneSum));
+    a.sums = ceil_div(blocks, a.sum_rest);
+    a.chain = ceil_div(a.sum_rest, chains);
+  } else if (blocks > kOneSum) {
+    a.sum_first = std::min(kSumBlocks, ceil_div(blocks, 2));
+    const int rest = blocks - 2 * a.sum_first, others = ceil_div(std::max(rest, 0), kSumBlocks);
+    a.sum_rest = others > 0 ? ceil_div(rest, others) : 1;
+    a.sums = 2 + others;
+  }
+}
+
 GemmArgs base_args(const HeadLossState& s) {
   GemmArgs a{};
   a.count = s.count;
@@ -1855,12 +1915,6 @@ GemmArgs base_args(const HeadLossState& s) {
   // us where chains of neighbours take 226 (64 rows of 3584 on 152064 columns).
   a.chain = ceil_div(ceil_div(s.H, kBK), most_chains(a.bn));
   a.chains = ceil_div(ceil_div(s.H, kBK), a.chain);
-  // the issuer makes as many sums as the epilogue takes: two of sum_first blocks, others of sum_rest, none empty
-  const int blocks = ceil_div(s.H, kBK);
-  a.sum_first = blocks <= kOneSum ? blocks : std::min(kSumBlocks, ceil_div(blocks, 2));
-  const int others = ceil_div(std::max(blocks - 2 * a.sum_first, 0), kSumBlocks);
-  a.sum_rest = others > 0 ? ceil_div(blocks - 2 * a.sum_first, others) : 1;
-  a.sums = std::min(blocks, 2 * a.sum_first) > a.sum_first ? 2 + others : 1;
   a.lo = ceil_div(s.R, 64) * 64;
   a.status = s.status;
   return a;
@@ -1963,6 +2017,7 @@ cudaError_t head_loss_forward_launch(const HeadLossState& s, const HeadStatsScra
   a.part = p.part;
   a.part_sum = p.part_sum;
   a.part_tiles = p.tiles;
+  cut_sums(a, few);
   cudaError_t e;
   if (few) {
     a.kept = p.kept != nullptr;
@@ -1973,7 +2028,8 @@ cudaError_t head_loss_forward_launch(const HeadLossState& s, const HeadStatsScra
     if (!map_bf16(&maps.a0, s.w, s.V, s.H, s.ldw, kBK, a.slot) ||
         !map_bf16(&maps.b0, s.hc, s.rpad, s.H, s.H, kBK, a.bn / 2))
       return cudaErrorInvalidValue;
-    e = launch_gemm<kStats, true>(maps, a, ceil_div(s.V, 2 * a.slot), stream);
+    const int items = ceil_div(s.V, 2 * a.slot);
+    e = a.sums > 1 ? launch_gemm<kStats, true, true>(maps, a, items, stream) : launch_gemm<kStats, true>(maps, a, items, stream);
   } else {
     if (!map_bf16(&maps.a0, s.hc, s.rpad, s.H, s.H, kBK, kHalf) || !map_bf16(&maps.b0, s.w, s.V, s.H, s.ldw, kBK, kHalf))
       return cudaErrorInvalidValue;
