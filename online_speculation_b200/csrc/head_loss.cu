@@ -52,8 +52,9 @@ constexpr int kMaxStages = 12;
 // into sums of at most kSumBlocks, which the epilogue adds in fp32.  The first two are the longest: while they are
 // multiplied, the exponentials of the tile before are formed.  Divergence losses of 300 rows of 3584, off by 3.8e-6 in one sum:
 // 5.3e-7 (6.2e-7 with fp32 products); the pass over 4096 rows of 3584 and 152064 columns 3.67 ms for 3.50 (sums of 14 blocks 3.60, of 8 3.83).
-// 14 blocks in one sum are off by 9e-7 at most.
-constexpr int kSumBlocks = 10, kOneSum = 14;
+// 300 rows of 896 in one sum 9.2e-7, in two 4.2e-7 (3.2e-7); the pass over 2048 rows of 896 and 65536 columns 0.263 ms for
+// 0.240.  Rows in columns: chains of at most kChainBlocks, 64 rows of 3584 6.9e-7 (7.3e-7).
+constexpr int kSumBlocks = 10, kOneSum = 12, kChainBlocks = 14;
 constexpr int kRowBytes = kBK * 2;        // one staged row of either operand
 constexpr int kBox = 64 * 64 * 2;         // one MN-major box: 64 reduction rows of 64 elements
 constexpr int kOutBytes = 32 * 128;       // one warp's staged output box: 32 rows of 128 bytes
@@ -1887,9 +1888,9 @@ void cut_sums(GemmArgs& a, bool few) {
   a.sums = 1;
   a.sum_first = a.sum_rest = blocks;
   if (few) {
-    if (a.chain <= kOneSum) return;
+    if (a.chain <= kChainBlocks) return;
     const int chains = most_chains(a.bn);
-    a.sum_first = a.sum_rest = ceil_div(blocks, ceil_div(blocks, chains * kOneSum));
+    a.sum_first = a.sum_rest = ceil_div(blocks, ceil_div(blocks, chains * kChainBlocks));
     a.sums = ceil_div(blocks, a.sum_rest);
     a.chain = ceil_div(a.sum_rest, chains);
   } else if (blocks > kOneSum) {

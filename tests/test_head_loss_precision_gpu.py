@@ -55,8 +55,8 @@ def test_gradients_of_short_lists(cuda, rows, hidden, vocab, k):
         assert _off(dw, want[4]) <= ONE_ROUNDING
 
 
-@pytest.mark.parametrize("rows,hidden", [(64, 3584), (64, 8192), (70, 2048), (128, 3584), (129, 3584), (192, 1536), (256, 3584), (300, 3584), (300, 1536),
-                                         (300, 2048), (513, 4096)])
+@pytest.mark.parametrize("rows,hidden", [(64, 3584), (64, 8192), (70, 2048), (128, 3584), (129, 3584), (192, 1536),
+                                         (256, 3584), (300, 3584), (300, 1536), (300, 896), (300, 2048), (513, 4096)])
 @pytest.mark.parametrize("listed", [0, 8])
 @pytest.mark.parametrize("kept", [False, True])
 def test_losses_are_summed_in_parts(cuda, rows, hidden, listed, kept):
