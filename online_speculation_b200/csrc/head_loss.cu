@@ -50,10 +50,11 @@ constexpr int kBK = 64;                   // reduction elements a stage: one 128
 constexpr int kMaxStages = 12;
 // Statistics of many rows: the tensor core truncates at every addition, so a reduction of more than kOneSum blocks is cut
 // into sums of at most kSumBlocks, which the epilogue adds in fp32.  The first two are the longest: while they are
-// multiplied, the exponentials of the tile before are formed.  Divergence losses of 300 rows of 3584, off by 3.8e-6 in one sum:
-// 5.3e-7 (6.2e-7 with fp32 products); the pass over 4096 rows of 3584 and 152064 columns 3.67 ms for 3.50 (sums of 14 blocks 3.60, of 8 3.83).
-// 300 rows of 896 in one sum 9.2e-7, in two 4.2e-7 (3.2e-7); the pass over 2048 rows of 896 and 65536 columns 0.263 ms for
-// 0.240.  Rows in columns: chains of at most kChainBlocks, 64 rows of 3584 6.9e-7 (7.3e-7).
+// multiplied, the exponentials of the tile before are formed.  Divergence losses of 300 rows of 3584, off by 3.8e-6 in
+// one sum: 5.3e-7 (6.2e-7 with fp32 products); the pass over 4096 rows of 3584 and 152064 columns 3.65 ms for 3.50 (sums
+// of 14 blocks 3.57, of 8 3.83).  300 rows of 896, off by 9.2e-7 in one sum: 4.2e-7 (3.2e-7); the pass over 2048 rows of
+// 896 and 65536 columns 0.261 ms for 0.240.  Rows in columns: chains of at most kChainBlocks, 64 rows of 3584 6.9e-7
+// (7.3e-7).
 constexpr int kSumBlocks = 10, kOneSum = 12, kChainBlocks = 14;
 constexpr int kRowBytes = kBK * 2;        // one staged row of either operand
 constexpr int kBox = 64 * 64 * 2;         // one MN-major box: 64 reduction rows of 64 elements
